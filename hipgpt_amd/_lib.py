@@ -33,6 +33,24 @@ _int = ctypes.c_int
 _vp = ctypes.c_void_p
 _f = ctypes.c_float
 
+_sz = ctypes.c_size_t
+
+
+class KvQ8Cache(ctypes.Structure):
+    """hipgpt_kvq8_cache of include/hipgpt_attn.h."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("page_stride", _i64),
+                ("head_stride", _i64), ("scale_page_stride", _i64), ("scale_head_stride", _i64), ("num_pages", _int),
+                ("page_size", _int), ("heads", _int), ("head_dim", _int)]
+
+
+class KvQ8Batch(ctypes.Structure):
+    """hipgpt_kvq8_batch of include/hipgpt_attn.h."""
+
+    _fields_ = [("block_table", _vp), ("table_stride", _i64), ("lens", _vp), ("cu_new", _vp), ("batch", _int),
+                ("max_pages", _int), ("max_new", _int)]
+
+
 SIGNATURES = {
     "hipgpt_attn_strerror": (ctypes.c_char_p, [_int]),
     "hipgpt_launch_multihead_attention": (None, [_vp, _vp, _vp, _int, _int, _int, _int]),
@@ -66,6 +84,16 @@ SIGNATURES = {
     "hipgpt_attn_wait_expired": (_int, [ctypes.POINTER(ctypes.c_uint), _int]),
     "hipgpt_attn_decode_default_splits": (_int, [_int, _int, _int]),
     "hipgpt_attn_decode_workspace_bytes": (ctypes.c_size_t, [_int, _int, _int, _int]),
+    "hipgpt_rope_freqs": (_int, [ctypes.POINTER(ctypes.c_uint64), _int, ctypes.c_double]),
+    "hipgpt_kvq8_append": (
+        _int, [_vp, _vp, _int] + [_vp] * 4 + [_int] + [_i64] * 8 + [_vp, _int, _int, _int, _int, _vp]),
+    "hipgpt_kvq8_read": (_int, [_vp, _vp, _int, _vp, _vp] + [_i64] * 4 + [_int, _vp]),
+    "hipgpt_attn_decode_kvq8_default_splits": (_int, [_int] * 4),
+    "hipgpt_attn_decode_kvq8_workspace_bytes": (_sz, [_int] * 4),
+    "hipgpt_attn_decode_kvq8": (
+        _int, [_vp, _vp, _vp, _vp, _int] + [_i64] * 4 + [_f, _int, _int, _int, _vp, _sz, _vp]),
+    "hipgpt_attn_prefill_kvq8": (
+        _int, [_vp, _vp, _int, _vp, _vp, _int] + [_i64] * 4 + [_f, _int, _int, _vp]),
     "hipgpt_attn_decode": (
         _int,
         [_vp, _vp, _vp, _vp, _int, _int, _int, _int]

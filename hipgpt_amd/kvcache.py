@@ -1,0 +1,249 @@
+"""Paged key/value cache in 8 bits over libhipgpt_attn.so (``include/hipgpt_attn.h``).
+
+HipGPT keeps no cache (its generation loop recomputes the window,
+``src/gpt_model.cpp:261-273``); :func:`hipgpt_amd.attention.decode_kvcache` keeps a
+contiguous fp32 one.  Here keys and values live in pages of 32, 64 or 128 tokens as
+8-bit codes with one scale per (page, head), query heads may share cached heads, and
+sequences of a batch bring ragged chunks of new tokens.
+
+* :class:`CacheQ8` -- the pools of one layer.
+* :class:`Batch` -- one step's sequences (pages, lengths, new tokens), for all layers.
+* :func:`append` -- rotate q and k by position, quantise k and v into the pages.
+* :func:`read` -- the values that cached tokens stand for.
+* :func:`decode` -- one query row per sequence, split over the keys.
+* :func:`prefill` -- a chunk of new tokens per sequence, causal.
+* :func:`rope_freqs` -- the rotation's frequencies.
+
+A step, in every layer: ``q = append(cache, batch, q, k, v, freqs=f)`` (``advance=True``
+in the first), then ``decode`` or ``prefill`` on that ``q``.  Nothing synchronises with
+the host; lengths and page tables are read on the device.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .attention import _need_cuda, _ptr
+
+_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _dtype(name, t):
+    dt = _TYPES.get(t if isinstance(t, torch.dtype) else t.dtype)
+    if dt is None:
+        raise TypeError(f"{name} must be float32 or bfloat16")
+    return dt
+
+
+class CacheQ8:
+    """Pools of one layer: ``k``, ``v`` uint8 [pages, heads, page_size, D] (the last two
+    dims contiguous; v's bytes are in the tile order of the header), ``k_scale``,
+    ``v_scale`` float32 [pages, heads]."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        for name, t, dt in (("k", k, torch.uint8), ("v", v, torch.uint8), ("k_scale", k_scale, torch.float32),
+                            ("v_scale", v_scale, torch.float32)):
+            _need_cuda(name, t, dt)
+            if t.device != k.device:
+                raise ValueError("the pools must be on one device")
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride():
+            raise ValueError("k, v must be [pages, heads, page_size, D] with the same strides")
+        P, H, ps, D = k.shape
+        if k.stride(3) != 1 or k.stride(2) != D:
+            raise ValueError("each (page, head) of k, v must be contiguous")
+        if tuple(k_scale.shape) != (P, H) or v_scale.shape != k_scale.shape or v_scale.stride() != k_scale.stride():
+            raise ValueError("k_scale, v_scale must be [pages, heads] with the same strides")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device, self.heads, self.page_size, self.head_dim = k.device, H, ps, D
+        self._c = _lib.KvQ8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                 k.stride(0), k.stride(1), k_scale.stride(0), k_scale.stride(1), P, ps, H, D)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, pages, heads, page_size, head_dim, device="cuda"):
+        """Pools without content (a page's scale is set by its first token)."""
+        codes = torch.empty(2, pages, heads, page_size, head_dim, dtype=torch.uint8, device=device)
+        scales = torch.empty(2, pages, heads, dtype=torch.float32, device=device)
+        return cls(codes[0], codes[1], scales[0], scales[1])
+
+
+class Batch:
+    """One step's sequences: ``block_table`` int32 [B, max_pages], ``lens`` int32 [B]
+    (tokens with the step's new ones), ``cu_new`` int32 [B + 1] (rows of the new tokens;
+    None: one each, row b), all on the device.  ``max_new``: the most new tokens of a
+    sequence; ``max_len``: a bound of ``lens`` that the default split goes by."""
+
+    def __init__(self, block_table, lens, cu_new=None, max_new=1, max_len=None):
+        _need_cuda("block_table", block_table, torch.int32)
+        _need_cuda("lens", lens, torch.int32)
+        if block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            raise ValueError("block_table must be [B, max_pages] with contiguous rows")
+        B, M = block_table.shape
+        if tuple(lens.shape) != (B,) or not lens.is_contiguous() or lens.device != block_table.device:
+            raise ValueError("lens must be a contiguous int32 tensor of B elements beside block_table")
+        if cu_new is not None:
+            _need_cuda("cu_new", cu_new, torch.int32)
+            if tuple(cu_new.shape) != (B + 1,) or not cu_new.is_contiguous() or cu_new.device != lens.device:
+                raise ValueError("cu_new must be a contiguous int32 tensor of B + 1 elements beside block_table")
+        elif max_new != 1:
+            raise ValueError("max_new is 1 without cu_new")
+        self.block_table, self.lens, self.cu_new = block_table, lens, cu_new  # kept alive
+        self.device, self.size, self.max_new = lens.device, B, int(max_new)
+        self.max_len = None if max_len is None else int(max_len)
+        self._c = _lib.KvQ8Batch(block_table.data_ptr(), block_table.stride(0), lens.data_ptr(), _ptr(cu_new), B, M,
+                                 self.max_new)
+        self._ref = ctypes.byref(self._c)
+
+    def capacity(self, cache):
+        """The most tokens a sequence's row of the table can hold."""
+        return self._c.max_pages * cache.page_size
+
+
+def rope_freqs(rot_dim, base=10000.0, device="cuda"):
+    """Turns per position of the ``rot_dim / 2`` rotated pairs as 0.64 fixed point
+    (int64 tensor), for :func:`append`."""
+    f = (ctypes.c_uint64 * max(1, rot_dim // 2))()
+    _lib.check(_lib.lib().hipgpt_rope_freqs(f, rot_dim, float(base)), "hipgpt_rope_freqs")
+    return torch.tensor(list(f), dtype=torch.int64, device=device)
+
+
+def _rows(name, t, T, heads, D, dtype, device):
+    """(token, head) strides of a [T, heads, D] tensor with contiguous D."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise TypeError(f"{name} must be a tensor on {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != (T, heads, D) or t.stride(2) != 1:
+        raise ValueError(f"{name} must be [{T}, {heads}, {D}] with contiguous D")
+    return t.stride(0), t.stride(1)
+
+
+def _call(cache, batch, name, make, stream, owned):
+    """Calls entry point ``name`` with ``make(stream handle)`` as arguments, on the cache's
+    device.  ``owned``: tensors allocated here, which another stream's kernels use."""
+    if batch.device != cache.device:
+        raise ValueError("cache and batch must be on one device")
+    if torch.cuda.current_device() != cache.device.index:
+        with torch.cuda.device(cache.device):
+            return _call(cache, batch, name, make, stream, owned)
+    if stream is None:
+        handle = torch.cuda.current_stream().cuda_stream
+    else:
+        handle = stream.cuda_stream
+        for t in owned:
+            t.record_stream(stream)
+    rc = getattr(_lib.lib(), name)(*make(handle))
+    if rc != _lib.OK:
+        _lib.check(rc, name)
+
+
+def append(cache, batch, q, k, v, freqs=None, interleaved=False, q_out=None, advance=False, stream=None):
+    """Rotates and quantises the new tokens into the cache; returns the rotated q.
+
+    k, v: [T, heads, D], q: [T, Hq, D] or None, all float32 or all bfloat16; ``freqs``:
+    :func:`rope_freqs` of the rotated head dims (None: no rotation); ``q_out`` may be q.
+    ``advance`` first raises ``batch.lens`` by the new tokens."""
+    dt = _dtype("k", k)
+    T, D, dev = k.shape[0], cache.head_dim, cache.device
+    ks = _rows("k", k, T, cache.heads, D, k.dtype, dev)
+    vs = _rows("v", v, T, cache.heads, D, k.dtype, dev)
+    Hq, qs, os_, owned = 0, (0, 0), (0, 0), ()
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError("q must be [T, Hq, D]")
+        Hq = q.shape[1]
+        qs = _rows("q", q, T, Hq, D, k.dtype, dev)
+        if q_out is None:
+            q_out = torch.empty((T, Hq, D), device=dev, dtype=k.dtype)
+            owned = (q_out,)
+        os_ = _rows("q_out", q_out, T, Hq, D, k.dtype, dev)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    rot = 0
+    if freqs is not None:
+        if freqs.dtype != torch.int64 or freqs.device != dev or freqs.dim() != 1 or not freqs.is_contiguous():
+            raise TypeError("freqs must be what rope_freqs gives, on the cache's device")
+        rot = 2 * freqs.numel()
+    _call(cache, batch, "hipgpt_kvq8_append", lambda s: (
+        cache._ref, batch._ref, T, _ptr(q), _ptr(q_out), k.data_ptr(), v.data_ptr(), Hq, *qs, *os_, *ks, *vs,
+        _ptr(freqs), rot, 1 if interleaved else 0, dt, 1 if advance else 0, s), stream, owned)
+    return q_out
+
+
+def read(cache, batch, T, dtype=torch.float32, k=None, v=None, stream=None):
+    """(k, v) [T, heads, D]: the values of each sequence's last ``cu_new[b + 1] -
+    cu_new[b]`` tokens, packed in that order (T rows in all)."""
+    shape = (T, cache.heads, cache.head_dim)
+    owned = []
+    if k is None:
+        k = torch.empty(shape, device=cache.device, dtype=dtype)
+        owned.append(k)
+    if v is None:
+        v = torch.empty(shape, device=cache.device, dtype=k.dtype)
+        owned.append(v)
+    dt = _dtype("k", k)
+    ks = _rows("k", k, *shape, k.dtype, cache.device)
+    vs = _rows("v", v, *shape, k.dtype, cache.device)
+    _call(cache, batch, "hipgpt_kvq8_read",
+          lambda s: (cache._ref, batch._ref, T, k.data_ptr(), v.data_ptr(), *ks, *vs, dt, s), stream, owned)
+    return k, v
+
+
+def _attention_args(cache, q, out, out_dtype):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q must be a [T, Hq, D] tensor")
+    T, Hq, D = q.shape
+    dt = _dtype("q", q)
+    owned = []
+    if out is None:
+        out = torch.empty((T, Hq, cache.head_dim), device=cache.device, dtype=out_dtype)
+        owned.append(out)
+    qs = _rows("q", q, T, Hq, cache.head_dim, q.dtype, cache.device)
+    os_ = _rows("out", out, T, Hq, cache.head_dim, out.dtype, cache.device)
+    return T, Hq, dt, _dtype("out", out), qs, os_, out, owned
+
+
+def decode_default_splits(B, Hq, heads, max_len):
+    return int(_lib.lib().hipgpt_attn_decode_kvq8_default_splits(B, Hq, heads, max_len))
+
+
+def decode_workspace_bytes(B, Hq, D, num_splits):
+    return int(_lib.lib().hipgpt_attn_decode_kvq8_workspace_bytes(B, Hq, D, num_splits))
+
+
+def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
+           stream=None):
+    """softmax(q k^T * scale) v of q [B, Hq, D] over each sequence's cached tokens.
+
+    float32 or bfloat16 q; ``out``: [B, Hq, D] float32, or bfloat16 for a bfloat16 q.
+    ``num_splits`` partitions of the keys (default: the library's choice for
+    ``batch.max_len``); ``workspace``: caller-owned (allocated here if None)."""
+    B, Hq, dt, odt, qs, os_, out, owned = _attention_args(cache, q, out, out_dtype)
+    if num_splits is None:
+        num_splits = decode_default_splits(B, Hq, cache.heads, batch.max_len or batch.capacity(cache))
+    if B != batch.size:
+        raise ValueError("q must have one row per sequence")
+    ns = max(1, min(int(num_splits), (batch.capacity(cache) + 31) // 32))
+    if workspace is None and ns > 1:
+        workspace = torch.empty(decode_workspace_bytes(B, Hq, cache.head_dim, ns), device=cache.device,
+                                dtype=torch.uint8)
+        owned.append(workspace)
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    sc = -1.0 if scale is None else float(scale)
+    _call(cache, batch, "hipgpt_attn_decode_kvq8",
+          lambda s: (cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, ns,
+                     _ptr(workspace), nbytes, s), stream, owned)
+    return out
+
+
+def prefill(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, stream=None):
+    """Causal attention of each sequence's new tokens (q [T, Hq, D], packed as
+    ``batch.cu_new``) over its cache, which holds them already."""
+    T, Hq, dt, odt, qs, os_, out, owned = _attention_args(cache, q, out, out_dtype)
+    sc = -1.0 if scale is None else float(scale)
+    _call(cache, batch, "hipgpt_attn_prefill_kvq8",
+          lambda s: (cache._ref, batch._ref, T, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, s),
+          stream, owned)
+    return out

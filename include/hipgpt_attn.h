@@ -178,6 +178,122 @@ int hipgpt_attn_decode_kvcache(const float* q, const float* k_new,
                                int num_splits, int advance, void* workspace,
                                size_t workspace_bytes, hipStream_t stream);
 
+/* ---- paged key/value cache in 8 bits ----
+ * No counterpart in HipGPT.  Keys and values live in pages of `page_size`
+ * tokens (32, 64 or 128) of one sequence, as codes u = c + 128 (c a whole
+ * number in [-127, 127]) with one fp32 scale per (page, head) for K and one
+ * for V; a value is c * scale.  heads: the cached heads; query heads are a
+ * multiple of them, query head x reads cached head x / (Hq / heads).
+ * head_dim D in {32, 64, 128, 256}.
+ *   k, v:    element (page, head) at X + page * page_stride + head *
+ *            head_stride, page_size * D bytes each; 16-byte aligned, strides
+ *            multiples of 16.  K is [token][D]; V is [token / 32][D / 32][4]
+ *            [16][2][2][4], where token % 32 = 16 i3 + 4 i0 + i4 and d % 32 =
+ *            16 i2 + i1 of the last five indexes i0 .. i4.
+ *   scales:  (page, head) at S[page * scale_page_stride + head *
+ *            scale_head_stride]; 2^-126 or more, or NaN for a page that was
+ *            given a value that is not finite.
+ * Memory of pages that no sequence holds is never read or written. */
+typedef struct hipgpt_kvq8_cache {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t page_stride, head_stride;
+    int64_t scale_page_stride, scale_head_stride;
+    int num_pages, page_size, heads, head_dim;
+} hipgpt_kvq8_cache;
+
+/* One step of a batch of sequences, shared by all layers.  All arrays are on
+ * the device and read there (no host synchronisation).
+ *   block_table: int [batch][max_pages] (row stride table_stride): the page
+ *                of tokens j * page_size .. of each sequence.
+ *   lens:        int [batch], tokens of each sequence, the step's new ones
+ *                included.
+ *   cu_new:      int [batch + 1]: sequence b's new tokens are rows cu_new[b]
+ *                .. cu_new[b + 1] - 1 of the packed buffers and positions
+ *                lens[b] - n .. lens[b] - 1.  NULL: one token each, row b
+ *                (then T = batch and max_new = 1).
+ *                lens[b] = 0 is then an empty slot: appends and reads skip
+ *                it, attention gives zeros.
+ *   max_new:     the most new tokens of any sequence.
+ * A sequence with lens[b] < n, more tokens than its table holds, or n >
+ * max_new is left as it is and gets NaN rows; so does what reads a page index
+ * outside [0, num_pages), which appends skip.  Rows that no sequence names
+ * (a cu_new that is not increasing or passes T) are left as they were.  Pages
+ * that several sequences hold may be read by all, and appended to by none. */
+typedef struct hipgpt_kvq8_batch {
+    const int* block_table;
+    int64_t table_stride;
+    int* lens;
+    const int* cu_new;
+    int batch, max_pages, max_new;
+} hipgpt_kvq8_batch;
+
+/* Host: turns per position of the rot_dim / 2 rotated pairs, base^(-2i /
+ * rot_dim) / 2 pi, as 0.64 fixed point.  base >= 1. */
+int hipgpt_rope_freqs(uint64_t* freqs, int rot_dim, double base);
+
+/* Appends the new tokens' keys and values, rotated by position on the way.
+ *   q, k, v: [T] rows of Hq / heads / heads head rows in `dtype`, element
+ *            (t, h, d) at X[t * x_ts + h * x_hs + d]; 16-byte aligned rows.
+ *   q_out:   receives the rotated q (may be q); q and q_out NULL: none.
+ *   freqs:   device [rot_dim / 2] as hipgpt_rope_freqs gives them: pair i of
+ *            position p turns by p * freqs[i] (exact at any position).  The
+ *            pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) where
+ *            interleaved; head dims from rot_dim on stay.  NULL: no rotation.
+ *   advance: non-zero first raises lens[b] by the sequence's new tokens (the
+ *            first layer's append of a step); 0: lens includes them already.
+ * Per (page, head) the new scale is max|x| / 127 over the page's new rows, at
+ * least 2^-126 and, where the page holds earlier tokens, at least their scale;
+ * where that grows, their codes are rounded again to the new one.  Codes are
+ * rounded to nearest even. */
+int hipgpt_kvq8_append(const hipgpt_kvq8_cache* cache,
+                       const hipgpt_kvq8_batch* batch, int T, const void* q,
+                       void* q_out, const void* k, const void* v, int Hq,
+                       int64_t q_ts, int64_t q_hs, int64_t qo_ts,
+                       int64_t qo_hs, int64_t k_ts, int64_t k_hs, int64_t v_ts,
+                       int64_t v_hs, const uint64_t* freqs, int rot_dim,
+                       int interleaved, int dtype, int advance,
+                       hipStream_t stream);
+
+/* The values that the last cu_new[b + 1] - cu_new[b] tokens of each sequence
+ * stand for, packed as the append takes them, in `dtype`. */
+int hipgpt_kvq8_read(const hipgpt_kvq8_cache* cache,
+                     const hipgpt_kvq8_batch* batch, int T, void* k, void* v,
+                     int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs,
+                     int dtype, hipStream_t stream);
+
+/* Attention of one query row per sequence (cu_new NULL) over its lens[b]
+ * cached tokens, split over the keys as hipgpt_attn_decode (num_splits <= 0
+ * picks the default for max_pages * page_size keys; the workspace is
+ * hipgpt_attn_decode_kvq8_workspace_bytes, NULL for one split).
+ *   q: in `dtype`, rotated already; o: in out_dtype; element (b, h, d) at
+ *   X[b * x_ts + h * x_hs + d], 16-byte aligned rows.  fp32 q takes fp32 o.
+ * Sums and softmax statistics are fp32.  With an fp32 result the products are
+ * off by 2^-22 of themselves at most; with a bf16 result the softmax weights
+ * are rounded to fp16 first.  An empty slot gives zeros. */
+int hipgpt_attn_decode_kvq8_default_splits(int B, int Hq, int heads,
+                                           int max_len);
+size_t hipgpt_attn_decode_kvq8_workspace_bytes(int B, int Hq, int D,
+                                               int num_splits);
+int hipgpt_attn_decode_kvq8(const hipgpt_kvq8_cache* cache,
+                            const hipgpt_kvq8_batch* batch, const void* q,
+                            void* o, int Hq, int64_t q_ts, int64_t q_hs,
+                            int64_t o_ts, int64_t o_hs, float scale, int dtype,
+                            int out_dtype, int num_splits, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
+/* Attention of a chunk of new tokens per sequence over its cache, which holds
+ * the chunk already: token i of n sees keys j <= lens[b] - n + i.  q, o as in
+ * hipgpt_attn_decode_kvq8, rows packed as cu_new says. */
+int hipgpt_attn_prefill_kvq8(const hipgpt_kvq8_cache* cache,
+                             const hipgpt_kvq8_batch* batch, int T,
+                             const void* q, void* o, int Hq, int64_t q_ts,
+                             int64_t q_hs, int64_t o_ts, int64_t o_hs,
+                             float scale, int dtype, int out_dtype,
+                             hipStream_t stream);
+
 /* Diagnostics, no counterpart in HipGPT.  One kernel synchronises its waves
  * through LDS flags instead of barriers (the one-workgroup-per-(b, h) backward
  * from lse at D = 32, S <= 256).
