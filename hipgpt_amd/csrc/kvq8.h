@@ -21,7 +21,8 @@
 namespace hipgpt {
 namespace kvq8 {
 
-constexpr int kTile = 32;  // tokens per V tile
+constexpr int kTile = 32;        // tokens per V tile
+constexpr int kMaxSplits = 1024;  // of the keys, or shares
 // Smallest scale: codes of values under it stay within [-127, 127] and its
 // reciprocal is finite.
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
@@ -105,15 +106,24 @@ struct AttnArgsQ8 {
     int Hq;
     float qscale;  // softmax scale * log2(e)
     int nsplit;
-    float* ws;  // nsplit > 1: (m, l) then O of each (row, split)
+    float* ws;  // nsplit > 1
 };
 
 bool supported(int D, int page_size);
 hipError_t launch_append(const Cache& c, const AppendArgs& a, int dtype, hipStream_t s);
 hipError_t launch_read(const Cache& c, const ReadArgs& a, int dtype, hipStream_t s);
 hipError_t launch_advance(int* lens, const int* cu, int B, hipStream_t s);
-int decode_splits(int B, int Hq, int Hkv, int max_len);
+// Attention of any number of rows.  Few rows per cached head (launch_rows in
+// kvq8_attn.hip) split the keys of each 16-row tile nsplit ways; more rows
+// (launch_tiles) take 128-row blocks, whole with nsplit 1, else as nsplit equal
+// shares of all their keys.
+bool tiles_for(int max_new, int G);
+int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int max_len);
+size_t attn_workspace(int T, int max_new, int Hq, int Hkv, int D, int nsplit);
 hipError_t launch_attn(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s);
+hipError_t launch_tiles(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s);
+int tile_shares(int D);
+size_t tile_workspace(int D, int shares);
 
 }  // namespace kvq8
 }  // namespace hipgpt

@@ -56,12 +56,24 @@ int problem(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, kvq8:
     return HIPGPT_OK;
 }
 
+// Both attention entry points.
 int attention(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, const void* q, void* o, int Hq,
-              int64_t q_ts, int64_t q_hs, int64_t o_ts, int64_t o_hs, float scale, int dtype, int out_dtype, int nsplit,
-              float* ws, hipStream_t stream) {
+              int64_t q_ts, int64_t q_hs, int64_t o_ts, int64_t o_hs, float scale, int dtype, int out_dtype,
+              int num_splits, void* ws, size_t ws_bytes, hipStream_t stream) {
     kvq8::Cache k{};
     const int rc = problem(c, b, T, k);
     if (rc != HIPGPT_OK) return rc;
+    if (!q || !o || Hq <= 0 || Hq % k.H != 0 || !std::isfinite(scale) || !is_dtype(dtype) || !is_dtype(out_dtype))
+        return HIPGPT_ERR_INVALID;
+    if (dtype == HIPGPT_F32 && out_dtype == HIPGPT_BF16) return HIPGPT_ERR_UNSUPPORTED;
+    if (!rows16(q, q_ts, q_hs, dtype) || !rows16(o, o_ts, o_hs, out_dtype)) return HIPGPT_ERR_UNSUPPORTED;
+    const int64_t cap = (int64_t)k.max_pages << k.lps;
+    int ns = num_splits > 0 ? num_splits
+                            : kvq8::attn_splits(k.B, k.T, k.max_new, Hq, k.H, k.D, cap > 0x7fffffff ? 0x7fffffff : (int)cap);
+    if (ns > kvq8::kMaxSplits) ns = kvq8::kMaxSplits;
+    const size_t need = kvq8::attn_workspace(k.T, k.max_new, Hq, k.H, k.D, ns);
+    if (need > 0 && (!ws || ws_bytes < need)) return HIPGPT_ERR_WORKSPACE;
+    if (need > 0 && !aligned(ws, 16)) return HIPGPT_ERR_UNSUPPORTED;
     kvq8::AttnArgsQ8 a{};
     a.q = q;
     a.o = o;
@@ -71,20 +83,9 @@ int attention(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, con
     a.o_hs = o_hs;
     a.Hq = Hq;
     a.qscale = (scale > 0.f ? scale : 1.0f / std::sqrt((float)k.D)) * kLog2e;
-    a.nsplit = nsplit;
-    a.ws = ws;
+    a.nsplit = ns;
+    a.ws = static_cast<float*>(ws);
     return from_hip(kvq8::launch_attn(k, a, dtype, out_dtype, stream));
-}
-
-// Checks that both attention entry points make before `problem`.
-int attention_args(const hipgpt_kvq8_cache* c, const void* q, const void* o, int Hq, int64_t q_ts, int64_t q_hs,
-                   int64_t o_ts, int64_t o_hs, float scale, int dtype, int out_dtype) {
-    if (!c || !q || !o || Hq <= 0 || c->heads <= 0 || Hq % c->heads != 0 || !std::isfinite(scale) ||
-        !is_dtype(dtype) || !is_dtype(out_dtype))
-        return HIPGPT_ERR_INVALID;
-    if (dtype == HIPGPT_F32 && out_dtype == HIPGPT_BF16) return HIPGPT_ERR_UNSUPPORTED;
-    if (!rows16(q, q_ts, q_hs, dtype) || !rows16(o, o_ts, o_hs, out_dtype)) return HIPGPT_ERR_UNSUPPORTED;
-    return HIPGPT_OK;
 }
 
 }  // namespace
@@ -153,41 +154,33 @@ int hipgpt_kvq8_read(const hipgpt_kvq8_cache* cache, const hipgpt_kvq8_batch* ba
     return from_hip(kvq8::launch_read(c, a, dtype, stream));
 }
 
-int hipgpt_attn_decode_kvq8_default_splits(int B, int Hq, int heads, int max_len) {
-    if (B <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || max_len <= 0) return 1;
-    return kvq8::decode_splits(B, Hq, heads, max_len);
+int hipgpt_attn_kvq8_default_splits(int B, int T, int max_new, int Hq, int heads, int D, int max_len) {
+    if (B <= 0 || T <= 0 || max_new <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0 || max_len <= 0)
+        return 1;
+    return kvq8::attn_splits(B, T, max_new < T ? max_new : T, Hq, heads, D, max_len);
 }
 
-size_t hipgpt_attn_decode_kvq8_workspace_bytes(int B, int Hq, int D, int num_splits) {
-    if (B <= 0 || Hq <= 0 || D <= 0 || num_splits <= 1) return 0;
-    return (size_t)B * Hq * num_splits * (size_t)(D + 2) * sizeof(float);
+size_t hipgpt_attn_kvq8_workspace_bytes(int T, int max_new, int Hq, int heads, int D, int num_splits) {
+    if (T <= 0 || max_new <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0) return 0;
+    return kvq8::attn_workspace(T, max_new < T ? max_new : T, Hq, heads, D,
+                                num_splits < kvq8::kMaxSplits ? num_splits : kvq8::kMaxSplits);
 }
 
 int hipgpt_attn_decode_kvq8(const hipgpt_kvq8_cache* cache, const hipgpt_kvq8_batch* batch, const void* q, void* o,
                             int Hq, int64_t q_ts, int64_t q_hs, int64_t o_ts, int64_t o_hs, float scale, int dtype,
                             int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
                             hipStream_t stream) {
-    const int rc = attention_args(cache, q, o, Hq, q_ts, q_hs, o_ts, o_hs, scale, dtype, out_dtype);
-    if (rc != HIPGPT_OK) return rc;
-    if (!batch || batch->cu_new || batch->max_new != 1 || batch->max_pages <= 0) return HIPGPT_ERR_INVALID;
-    const int64_t cap = (int64_t)batch->max_pages * cache->page_size;
-    int ns = num_splits > 0 ? num_splits
-                            : hipgpt_attn_decode_kvq8_default_splits(batch->batch, Hq, cache->heads,
-                                                                     cap > 0x7fffffff ? 0x7fffffff : (int)cap);
-    if (ns > (cap + kvq8::kTile - 1) / kvq8::kTile) ns = (int)((cap + kvq8::kTile - 1) / kvq8::kTile);
-    if (ns < 1) ns = 1;
-    const size_t need = hipgpt_attn_decode_kvq8_workspace_bytes(batch->batch, Hq, cache->head_dim, ns);
-    if (need > 0 && (!workspace || workspace_bytes < need)) return HIPGPT_ERR_WORKSPACE;
-    return attention(cache, batch, batch->batch, q, o, Hq, q_ts, q_hs, o_ts, o_hs, scale, dtype, out_dtype, ns,
-                     static_cast<float*>(workspace), stream);
+    if (!batch || batch->cu_new || batch->max_new != 1) return HIPGPT_ERR_INVALID;
+    return attention(cache, batch, batch->batch, q, o, Hq, q_ts, q_hs, o_ts, o_hs, scale, dtype, out_dtype, num_splits,
+                     workspace, workspace_bytes, stream);
 }
 
 int hipgpt_attn_prefill_kvq8(const hipgpt_kvq8_cache* cache, const hipgpt_kvq8_batch* batch, int T, const void* q,
                              void* o, int Hq, int64_t q_ts, int64_t q_hs, int64_t o_ts, int64_t o_hs, float scale,
-                             int dtype, int out_dtype, hipStream_t stream) {
-    const int rc = attention_args(cache, q, o, Hq, q_ts, q_hs, o_ts, o_hs, scale, dtype, out_dtype);
-    if (rc != HIPGPT_OK) return rc;
-    return attention(cache, batch, T, q, o, Hq, q_ts, q_hs, o_ts, o_hs, scale, dtype, out_dtype, 1, nullptr, stream);
+                             int dtype, int out_dtype, int num_splits, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream) {
+    return attention(cache, batch, T, q, o, Hq, q_ts, q_hs, o_ts, o_hs, scale, dtype, out_dtype, num_splits, workspace,
+                     workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -25,30 +25,15 @@
 // one number for all rows, so a page costs one multiplication per score.
 #include "common.h"
 #include "kernels.h"
-#include "kvq8.h"
+#include "kvq8_attn.h"
 
 namespace hipgpt {
 namespace kvq8 {
 
 namespace {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-
 constexpr int NW = 4;            // waves per workgroup
 constexpr float kPShift = 15.f;  // p is kept as p * 2^15: fp16 then holds 2^-39 .. 1
-
-// Two codes of word w as fp16 numbers.
-template <int HI>
-__device__ __forceinline__ half2v codes2(unsigned w) {
-    const unsigned x = __builtin_amdgcn_perm(0x64646464u, w, HI ? 0x04030402u : 0x04010400u);
-    const half2v bias = {(_Float16)1152.f, (_Float16)1152.f};
-    return __builtin_bit_cast(half2v, x) - bias;
-}
-__device__ __forceinline__ half8 codes8(unsigned w0, unsigned w1) {
-    const half2v a = codes2<0>(w0), b = codes2<1>(w0), c = codes2<0>(w1), d = codes2<1>(w1);
-    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 __device__ __forceinline__ float xor8_add(float x) {  // + the lane 8 places away in its row of 16
     const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false);
@@ -62,9 +47,6 @@ __device__ __forceinline__ float col_max(float x) {
 __device__ __forceinline__ float col_sum(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
-}
-__device__ __forceinline__ float lane_value(float x, int lane) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
 // Raw codes of one 32-token tile of one head.
@@ -96,35 +78,6 @@ __device__ __forceinline__ void load_tile(Tile<D>& t, const uint8_t* kp, const u
 template <int D>
 __device__ __forceinline__ int q_dim(int s, int q) {
     return D == 32 ? q * 8 : (s >> 1) * 64 + q * 16 + (s & 1) * 8;
-}
-
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float* x);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* x) {
-    const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        x[j] = a[j];
-        x[4 + j] = b[j];
-    }
-}
-template <>
-__device__ __forceinline__ void load8<__bf16>(const __bf16* p, float* x) {
-    const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)a[j];
-}
-
-// 2^e and 2^-e with x * 2^e in [2^13, 2^14) for the largest |x| of a row
-// (1 where that is 0 or not finite).
-__device__ __forceinline__ void row_scale(float amax, float& up, float& down) {
-    const int e = (int)(__float_as_uint(amax) >> 23);  // biased exponent
-    up = down = 1.f;
-    if (e == 255 || amax == 0.f) return;
-    const int k = min(13 - (e - 127), 126);
-    up = __uint_as_float((unsigned)(127 + k) << 23);
-    down = __uint_as_float((unsigned)(127 - k) << 23);
 }
 
 // One workgroup: 16 / TERMS rows of one (sequence, cached head), one split of
@@ -186,24 +139,12 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_kernel(Cache c, AttnArgsQ8 
     for (int i = 0; i < D / 16; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = kMaxInit, l = 0.f, ref = 0.f;
 
-    int meta_page = 0;
-    float meta_ks = 0.f, meta_vs = 0.f;
+    TileMeta meta;
     int cnt = 0;
     for (int t = tile0 + wave; t < tile1; t += NW, ++cnt) {
-        if ((cnt & 63) == 0) {  // page and scales of this wave's next 64 tiles, one a lane
-            const int mt = t + lane * NW;
-            meta_page = 0;
-            meta_ks = meta_vs = 0.f;
-            if (mt < tile1) {
-                const int p = page_of(c, b, mt * kTile);
-                meta_page = max(p, 0);
-                const int64_t at = meta_page * c.s_page_stride + h * c.s_head_stride;
-                meta_ks = p < 0 ? __builtin_nanf("") : c.ks[at];
-                meta_vs = p < 0 ? __builtin_nanf("") : c.vs[at];
-            }
-        }
-        const int page = __builtin_amdgcn_readlane(meta_page, cnt & 63);
-        const float ks = lane_value(meta_ks, cnt & 63), vs = lane_value(meta_vs, cnt & 63);
+        if ((cnt & 63) == 0) meta.load(c, b, h, t, NW, tile1, lane);
+        const int page = __builtin_amdgcn_readlane(meta.page, cnt & 63);
+        const float ks = lane_value(meta.ks, cnt & 63), vs = lane_value(meta.vs, cnt & 63);
         const int tok = (t * kTile) & ((1 << c.lps) - 1);
         const int64_t at = (int64_t)page * c.page_stride + (int64_t)h * c.head_stride + tok * D;
         Tile<D> tl;
@@ -303,27 +244,76 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_kernel(Cache c, AttnArgsQ8 
     }
 }
 
-// Joins the splits of one (row, head): O = sum_s O_s L_s 2^(m_s - M) / sum_s L_s 2^(m_s - M).
-template <int D, class TO>
+// Joins the splits of rows: O = sum_s O_s L_s 2^(m_s - M) / sum_s L_s 2^(m_s - M).
+// D / 4 lanes (four head dims each) and PAR of them side by side per row: the
+// split rows of one row are loaded PAR at a time, since each load waits for
+// memory that another XCD wrote.  A workgroup of 256 takes 256 / (PAR D / 4) rows.
+template <int D, int PAR, class TO>
 __global__ __launch_bounds__(256) void attn_join_kernel(Cache c, AttnArgsQ8 a) {
-    const int h = blockIdx.x % a.Hq, bi = blockIdx.x / a.Hq;
-    const Seq q = sequence(c, bi / c.max_new);
-    if (bi % c.max_new >= q.n) return;
-    const int64_t row = q.row0 + bi % c.max_new;
-    const int64_t slot = (row * a.Hq + h) * a.nsplit;
-    const float* ml = a.ws + 2 * slot;
-    const float* po = a.ws + 2 * (int64_t)c.T * a.Hq * a.nsplit + slot * D;
-    float M = kMaxInit;
-    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, ml[2 * s]);
-    const int d = threadIdx.x;
-    float L = 0.f, O = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float w = ml[2 * s + 1] * fast_exp2(ml[2 * s] - M);
-        L += w;
-        if (d < D) O += w == 0.f ? 0.f : w * po[(int64_t)s * D + d];
+    constexpr int LP = D / 4;            // lanes per split row
+    constexpr int TPR = LP * PAR;        // threads per row
+    constexpr int RPW = 256 / TPR;       // rows per workgroup
+    __shared__ __attribute__((aligned(16))) float s_o[PAR > 1 ? 256 : 1][4];
+    __shared__ float s_l[PAR > 1 ? 256 : 1];
+    const int tid = threadIdx.x, sub = tid % LP, par = tid / LP % PAR;
+    const int64_t item = (int64_t)blockIdx.x * RPW + tid / TPR;  // (sequence, token, head)
+    const int h = (int)(item % a.Hq);
+    const int64_t bi = item / a.Hq;
+    bool live = bi < (int64_t)c.B * c.max_new;
+    int64_t row = 0;
+    if (live) {
+        const Seq q = sequence(c, (int)(bi / c.max_new));
+        live = bi % c.max_new < q.n;
+        row = q.row0 + bi % c.max_new;
     }
-    if (d < D)
-        static_cast<TO*>(a.o)[row * a.o_ts + h * a.o_hs + d] = (TO)(L > 0.f || L != L ? O / L : 0.f);
+    floatx4 O = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+    if (live) {
+        const int64_t slot = (row * a.Hq + h) * a.nsplit;
+        const float2* ml = reinterpret_cast<const float2*>(a.ws) + slot;
+        const float* po = a.ws + 2 * (int64_t)c.T * a.Hq * a.nsplit + slot * D + sub * 4;
+        float M = kMaxInit;
+        for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, ml[s].x);
+#pragma unroll 4
+        for (int s = par; s < a.nsplit; s += PAR) {
+            const float2 x = ml[s];
+            const float w = x.y * fast_exp2(x.x - M);
+            const floatx4 v = *reinterpret_cast<const floatx4*>(po + (int64_t)s * D);
+            L += w;
+            if (w != 0.f) O += w * v;
+        }
+    }
+    if constexpr (PAR > 1) {
+        *reinterpret_cast<floatx4*>(s_o[tid]) = O;
+        s_l[tid] = L;
+        __syncthreads();
+        if (par != 0) return;
+#pragma unroll
+        for (int g = 1; g < PAR; ++g) {
+            O += *reinterpret_cast<const floatx4*>(s_o[tid + g * LP]);
+            L += s_l[tid + g * LP];
+        }
+    }
+    if (!live) return;
+    TO* op = static_cast<TO*>(a.o) + row * a.o_ts + h * a.o_hs + sub * 4;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) op[v] = (TO)(L > 0.f || L != L ? O[v] / L : 0.f);
+}
+
+template <int D, int PAR, class TO>
+hipError_t launch_join_t(const Cache& c, const AttnArgsQ8& a, hipStream_t s) {
+    constexpr int RPW = 256 / (D / 4 * PAR);
+    const int64_t grid = ((int64_t)c.B * c.max_new * a.Hq + RPW - 1) / RPW;
+    if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((attn_join_kernel<D, PAR, TO>), dim3((unsigned)grid), dim3(256), 0, s, c, a);
+    return hipGetLastError();
+}
+
+template <int D, class TO>
+hipError_t launch_join(const Cache& c, const AttnArgsQ8& a, hipStream_t s) {
+    // few splits: a row needs no help; many: as many lanes as a workgroup has
+    if (a.nsplit <= 4) return launch_join_t<D, 1, TO>(c, a, s);
+    return launch_join_t<D, 1024 / D, TO>(c, a, s);
 }
 
 template <int D, int TERMS, class TI, class TO>
@@ -331,29 +321,47 @@ hipError_t launch_rows(const Cache& c, const AttnArgsQ8& a, hipStream_t s) {
     const int rpb = 16 / TERMS;
     const int64_t row_blocks = ((int64_t)c.max_new * (a.Hq / c.H) + rpb - 1) / rpb;
     const int64_t grid = row_blocks * c.H * c.B * a.nsplit;
-    if (grid <= 0 || grid > 0x7fffffff || (int64_t)c.B * c.max_new * a.Hq > 0x7fffffff) return hipErrorInvalidConfiguration;
+    if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((attn_rows_kernel<D, TERMS, TI, TO>), dim3((unsigned)grid), dim3(NW * 64), 0, s, c, a,
                        (int)row_blocks);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.nsplit == 1) return e;
-    hipLaunchKernelGGL((attn_join_kernel<D, TO>), dim3((unsigned)(c.B * c.max_new * a.Hq)), dim3(D < 64 ? 64 : D), 0, s, c, a);
     return hipGetLastError();
 }
 
 template <int D>
 hipError_t launch_dim(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s) {
-    if (dtype == kF32) return launch_rows<D, 2, float, float>(c, a, s);
-    if (out_dtype == kF32) return launch_rows<D, 2, __bf16, float>(c, a, s);
-    return launch_rows<D, 1, __bf16, __bf16>(c, a, s);
+        hipError_t e;
+    if (tiles_for(c.max_new, a.Hq / c.H)) return launch_tiles(c, a, dtype, out_dtype, s);
+    if (dtype == kF32)
+        e = launch_rows<D, 2, float, float>(c, a, s);
+    else if (out_dtype == kF32)
+        e = launch_rows<D, 2, __bf16, float>(c, a, s);
+    else
+        e = launch_rows<D, 1, __bf16, __bf16>(c, a, s);
+    if (e != hipSuccess || a.nsplit == 1) return e;
+    return out_dtype == kF32 ? launch_join<D, float>(c, a, s) : launch_join<D, __bf16>(c, a, s);
 }
 
 }  // namespace
 
-int decode_splits(int B, int Hq, int Hkv, int max_len) {
-    const int64_t wgs = (int64_t)B * Hkv * ((Hq / Hkv + 15) / 16);
+// Whether so many rows of one cached head take the 128-row blocks.
+bool tiles_for(int max_new, int G) { return (int64_t)max_new * G > 32; }
+
+int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int max_len) {
+    const int64_t G = Hq / Hkv;
+    if (tiles_for(max_new, (int)G)) {
+        const int64_t blocks = Hkv * (T * G / 128 + B);  // row blocks, at most
+        return blocks < tile_shares(D) && max_len >= 1024 ? tile_shares(D) : 1;
+    }
+    const int64_t wgs = Hkv * B * ((max_new * G + 15) / 16);
     int n = 1;
-    while (n < 128 && wgs * n <= 512 && max_len / (2 * n) >= 256) n *= 2;
+    while (n < 256 && wgs * n <= 512 && max_len / (2 * n) >= 256) n *= 2;
     return n;
+}
+
+size_t attn_workspace(int T, int max_new, int Hq, int Hkv, int D, int nsplit) {
+    if (nsplit <= 1) return 0;
+    if (tiles_for(max_new, Hq / Hkv)) return tile_workspace(D, nsplit);
+    return (size_t)T * Hq * nsplit * (size_t)(D + 2) * sizeof(float);
 }
 
 hipError_t launch_attn(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s) {

@@ -205,12 +205,25 @@ def _attention_args(cache, q, out, out_dtype):
     return T, Hq, dt, _dtype("out", out), qs, os_, out, owned
 
 
-def decode_default_splits(B, Hq, heads, max_len):
-    return int(_lib.lib().hipgpt_attn_decode_kvq8_default_splits(B, Hq, heads, max_len))
+def default_splits(B, T, max_new, Hq, heads, D, max_len):
+    return int(_lib.lib().hipgpt_attn_kvq8_default_splits(B, T, max_new, Hq, heads, D, max_len))
 
 
-def decode_workspace_bytes(B, Hq, D, num_splits):
-    return int(_lib.lib().hipgpt_attn_decode_kvq8_workspace_bytes(B, Hq, D, num_splits))
+def workspace_bytes(T, max_new, Hq, heads, D, num_splits):
+    return int(_lib.lib().hipgpt_attn_kvq8_workspace_bytes(T, max_new, Hq, heads, D, num_splits))
+
+
+def _splits(cache, batch, T, Hq, num_splits, workspace, owned):
+    """(split count, workspace, its bytes) of an attention call."""
+    H, D = cache.heads, cache.head_dim
+    if num_splits is None:
+        num_splits = default_splits(batch.size, T, batch.max_new, Hq, H, D, batch.max_len or batch.capacity(cache))
+    ns = max(1, int(num_splits))
+    if workspace is None and ns > 1:
+        workspace = torch.empty(workspace_bytes(T, batch.max_new, Hq, H, D, ns), device=cache.device,
+                                dtype=torch.uint8)
+        owned.append(workspace)
+    return ns, _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size()
 
 
 def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
@@ -218,32 +231,29 @@ def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_s
     """softmax(q k^T * scale) v of q [B, Hq, D] over each sequence's cached tokens.
 
     float32 or bfloat16 q; ``out``: [B, Hq, D] float32, or bfloat16 for a bfloat16 q.
-    ``num_splits`` partitions of the keys (default: the library's choice for
-    ``batch.max_len``); ``workspace``: caller-owned (allocated here if None)."""
+    ``num_splits`` partitions of the work (default: the library's choice for
+    ``batch.max_len``); ``workspace``: caller-owned, :func:`workspace_bytes` (allocated
+    here if None)."""
     B, Hq, dt, odt, qs, os_, out, owned = _attention_args(cache, q, out, out_dtype)
-    if num_splits is None:
-        num_splits = decode_default_splits(B, Hq, cache.heads, batch.max_len or batch.capacity(cache))
     if B != batch.size:
         raise ValueError("q must have one row per sequence")
-    ns = max(1, min(int(num_splits), (batch.capacity(cache) + 31) // 32))
-    if workspace is None and ns > 1:
-        workspace = torch.empty(decode_workspace_bytes(B, Hq, cache.head_dim, ns), device=cache.device,
-                                dtype=torch.uint8)
-        owned.append(workspace)
-    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    ns, ws, nbytes = _splits(cache, batch, B, Hq, num_splits, workspace, owned)
     sc = -1.0 if scale is None else float(scale)
     _call(cache, batch, "hipgpt_attn_decode_kvq8",
-          lambda s: (cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, ns,
-                     _ptr(workspace), nbytes, s), stream, owned)
+          lambda s: (cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, ns, ws, nbytes,
+                     s), stream, owned)
     return out
 
 
-def prefill(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, stream=None):
+def prefill(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
+            stream=None):
     """Causal attention of each sequence's new tokens (q [T, Hq, D], packed as
-    ``batch.cu_new``) over its cache, which holds them already."""
+    ``batch.cu_new``) over its cache, which holds them already.  The rest as
+    :func:`decode`."""
     T, Hq, dt, odt, qs, os_, out, owned = _attention_args(cache, q, out, out_dtype)
+    ns, ws, nbytes = _splits(cache, batch, T, Hq, num_splits, workspace, owned)
     sc = -1.0 if scale is None else float(scale)
     _call(cache, batch, "hipgpt_attn_prefill_kvq8",
-          lambda s: (cache._ref, batch._ref, T, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, s),
-          stream, owned)
+          lambda s: (cache._ref, batch._ref, T, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, ns, ws,
+                     nbytes, s), stream, owned)
     return out

@@ -264,35 +264,44 @@ int hipgpt_kvq8_read(const hipgpt_kvq8_cache* cache,
                      int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs,
                      int dtype, hipStream_t stream);
 
-/* Attention of one query row per sequence (cu_new NULL) over its lens[b]
- * cached tokens, split over the keys as hipgpt_attn_decode (num_splits <= 0
- * picks the default for max_pages * page_size keys; the workspace is
- * hipgpt_attn_decode_kvq8_workspace_bytes, NULL for one split).
- *   q: in `dtype`, rotated already; o: in out_dtype; element (b, h, d) at
- *   X[b * x_ts + h * x_hs + d], 16-byte aligned rows.  fp32 q takes fp32 o.
+/* Attention over the cache.
+ *   decode:  one query row per sequence (cu_new NULL), over its lens[b]
+ *            tokens.  An empty slot gives zeros.
+ *   prefill: the new tokens of each sequence (T rows, packed as cu_new says);
+ *            the cache holds them already, token i of n sees keys
+ *            j <= lens[b] - n + i.
+ *   q: in `dtype`, rotated already; o: in out_dtype; element (row, h, d) at
+ *   X[row * x_ts + h * x_hs + d], 16-byte aligned rows.  An fp32 q takes an
+ *   fp32 o.  scale <= 0 selects 1/sqrt(D).
+ * num_splits > 1 divides the work and joins the parts by a second kernel
+ * through a caller-owned, 16-byte aligned workspace of
+ * hipgpt_attn_kvq8_workspace_bytes: up to 32 query rows per cached head and
+ * sequence (max_new * Hq / heads), each row's keys num_splits ways; with more,
+ * the keys of all blocks of 128 rows in num_splits equal shares.  At most
+ * 1024; <= 0: hipgpt_attn_kvq8_default_splits for max_len = max_pages *
+ * page_size (T = batch in decode).  1 needs no workspace.
  * Sums and softmax statistics are fp32.  With an fp32 result the products are
  * off by 2^-22 of themselves at most; with a bf16 result the softmax weights
- * are rounded to fp16 first.  An empty slot gives zeros. */
-int hipgpt_attn_decode_kvq8_default_splits(int B, int Hq, int heads,
-                                           int max_len);
-size_t hipgpt_attn_decode_kvq8_workspace_bytes(int B, int Hq, int D,
-                                               int num_splits);
+ * are rounded to fp16 first.  V scales are applied to those weights relative
+ * to the largest scale that the row's block of rows met, so what pages with
+ * scales under 2^-24 of it contribute is lost in part (fp16's range). */
+int hipgpt_attn_kvq8_default_splits(int B, int T, int max_new, int Hq,
+                                    int heads, int D, int max_len);
+size_t hipgpt_attn_kvq8_workspace_bytes(int T, int max_new, int Hq, int heads,
+                                        int D, int num_splits);
 int hipgpt_attn_decode_kvq8(const hipgpt_kvq8_cache* cache,
                             const hipgpt_kvq8_batch* batch, const void* q,
                             void* o, int Hq, int64_t q_ts, int64_t q_hs,
                             int64_t o_ts, int64_t o_hs, float scale, int dtype,
                             int out_dtype, int num_splits, void* workspace,
                             size_t workspace_bytes, hipStream_t stream);
-
-/* Attention of a chunk of new tokens per sequence over its cache, which holds
- * the chunk already: token i of n sees keys j <= lens[b] - n + i.  q, o as in
- * hipgpt_attn_decode_kvq8, rows packed as cu_new says. */
 int hipgpt_attn_prefill_kvq8(const hipgpt_kvq8_cache* cache,
                              const hipgpt_kvq8_batch* batch, int T,
                              const void* q, void* o, int Hq, int64_t q_ts,
                              int64_t q_hs, int64_t o_ts, int64_t o_hs,
                              float scale, int dtype, int out_dtype,
-                             hipStream_t stream);
+                             int num_splits, void* workspace,
+                             size_t workspace_bytes, hipStream_t stream);
 
 /* Diagnostics, no counterpart in HipGPT.  One kernel synchronises its waves
  * through LDS flags instead of barriers (the one-workgroup-per-(b, h) backward

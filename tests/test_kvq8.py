@@ -84,7 +84,7 @@ def calls(c, b, T):
     s = (128, 64)
     yield L.hipgpt_kvq8_append(c, b, T, P, P, P, P, 2, *s, *s, *s, *s, P, 64, 0, 0, 0, None)
     yield L.hipgpt_kvq8_read(c, b, T, P, P, *s, *s, 0, None)
-    yield L.hipgpt_attn_prefill_kvq8(c, b, T, P, P, 2, *s, *s, -1.0, 0, 0, None)
+    yield L.hipgpt_attn_prefill_kvq8(c, b, T, P, P, 2, *s, *s, -1.0, 0, 0, 1, None, 0, None)
 
 
 BAD_CACHES = [
@@ -151,7 +151,7 @@ def test_attention_refusals():
 
     def both(q=P, o=P, Hq=4, qs=s, os_=s, scale=-1.0, dt=0, odt=0, c=None):
         c = c or cache()
-        pre = L.hipgpt_attn_prefill_kvq8(c, batch(), 7, q, o, Hq, *qs, *os_, scale, dt, odt, None)
+        pre = L.hipgpt_attn_prefill_kvq8(c, batch(), 7, q, o, Hq, *qs, *os_, scale, dt, odt, 1, None, 0, None)
         dec = L.hipgpt_attn_decode_kvq8(c, batch(cu_new=0, max_new=1), q, o, Hq, *qs, *os_, scale, dt, odt, 1, None, 0,
                                         None)
         assert pre == dec
@@ -170,13 +170,27 @@ def test_attention_refusals():
     assert dec(cache(), None, P, P, 4, *s, *s, -1.0, 0, 0, 1, None, 0, None) == _lib.ERR_INVALID
     assert dec(None, batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 1, None, 0, None) == _lib.ERR_INVALID
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, None, 0, None) == _lib.ERR_WORKSPACE
-    need = L.hipgpt_attn_decode_kvq8_workspace_bytes(2, 4, 64, 3)
+    wb = L.hipgpt_attn_kvq8_workspace_bytes
+    need = wb(2, 1, 4, 2, 64, 3)
     assert need == 2 * 4 * 3 * 66 * 4
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, P, need - 4, None) == _lib.ERR_WORKSPACE
-    assert L.hipgpt_attn_decode_kvq8_workspace_bytes(2, 4, 64, 1) == 0
-    assert L.hipgpt_attn_decode_kvq8_default_splits(2, 5, 4, 1 << 20) == 1  # heads that do not divide
-    assert L.hipgpt_attn_decode_kvq8_default_splits(1, 8, 8, 100) == 1
-    assert L.hipgpt_attn_decode_kvq8_default_splits(1, 8, 8, 1 << 17) >= 16
+    assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, P + 4, need, None) == _lib.ERR_UNSUPPORTED
+    assert wb(2, 1, 4, 2, 64, 1) == wb(0, 1, 4, 2, 64, 4) == wb(2, 1, 5, 2, 64, 4) == 0
+    assert wb(2, 1, 4, 2, 64, 5000) == wb(2, 1, 4, 2, 64, 1024)
+    pre = L.hipgpt_attn_prefill_kvq8
+    # 10 rows of a cached head: split rows; 100: shares of 128-row blocks, two slots each
+    need = wb(7, 5, 4, 2, 64, 2)
+    assert need == 7 * 4 * 2 * 66 * 4
+    assert pre(cache(), batch(), 7, P, P, 4, *s, *s, -1.0, 0, 0, 2, P, need - 4, None) == _lib.ERR_WORKSPACE
+    need = wb(70, 50, 4, 2, 64, 3)
+    assert need == 3 * (4 + 2 * 128 * (64 + 4)) * 4
+    assert pre(cache(), batch(max_new=50), 70, P, P, 4, *s, *s, -1.0, 0, 0, 3, P, need - 4, None) == _lib.ERR_WORKSPACE
+    ds = L.hipgpt_attn_kvq8_default_splits
+    assert ds(2, 2, 1, 5, 4, 64, 1 << 20) == 1  # heads that do not divide
+    assert ds(0, 2, 1, 4, 4, 64, 99999) == ds(2, 0, 1, 4, 4, 64, 99999) == ds(2, 2, 0, 4, 4, 64, 99999) == 1
+    assert ds(1, 1, 1, 8, 8, 64, 100) == 1
+    assert 16 <= ds(1, 1, 1, 8, 8, 64, 1 << 17) <= 256
+    assert ds(1, 4096, 4096, 8, 8, 128, 1 << 15) == 512 and ds(64, 65536, 1024, 8, 8, 128, 1024) == 1 == ds(1, 500, 500, 8, 8, 128, 1000)
 
 
 def test_python_wrappers_refuse_host_tensors():

@@ -357,8 +357,9 @@ def test_prefill(dev, D, G, dtype, out):
     H, ps = 2, 64
     c = Case(D + G, lens, lens, H, ps, D, pad=16)
     q, q64 = normal(c.rng, dtype, sum(new), G * H, D)
-    got = host(K.prefill(c.cache, c.batch(lens, new), q, out_dtype=DT[out]))
-    check_attention(c, got, q64, lens, new, G, D**-0.5, out)
+    for splits in (1, 3, 40, None):
+        got = host(K.prefill(c.cache, c.batch(lens, new), q, out_dtype=DT[out], num_splits=splits))
+        check_attention(c, got, q64, lens, new, G, D**-0.5, out)
 
 
 @pytest.mark.parametrize("ps", [32, 128])
@@ -444,12 +445,13 @@ def test_prefill_does_not_see_what_is_behind(dev, dtype, out):
     c.cache.v_scale[int(c.table[0, 2])] = float("nan")
     c.cache.k_scale[int(c.table[0, 1])] = float("nan")
     q, q64 = normal(c.rng, dtype, n, 2, D)
-    got = host(K.prefill(c.cache, c.batch([n], [n]), q, out_dtype=DT[out]))
-    assert np.isnan(got[32:]).all()
     k, v = c.rows("k", 0, 32), c.rows("v", 0, 32)
     want = R.attend(q64[:32], k, v, 2, D**-0.5, 0)
     tol = R.f32_tol(v) if out == "f32" else R.bf16_tol(want, v)
-    assert (np.abs(got[:32] - want) <= tol).all()
+    for splits in (1, 3):
+        got = host(K.prefill(c.cache, c.batch([n], [n]), q, out_dtype=DT[out], num_splits=splits))
+        assert np.isnan(got[32:]).all()
+        assert (np.abs(got[:32] - want) <= tol).all()
 
 
 def test_rows_that_no_sequence_names_stay(dev):
@@ -544,7 +546,7 @@ def test_captured_steps_replay(dev):
     f = K.rope_freqs(D)
     q, k, v = (normal(c.rng, "f32", B, H, D)[0] for _ in range(3))
     out, out2, qr = (torch.empty(B, H, D, device="cuda") for _ in range(3))
-    ws = torch.empty(K.decode_workspace_bytes(B, H, D, 4), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(K.workspace_bytes(B, 1, H, H, D, 4), dtype=torch.uint8, device="cuda")
     lens = dev_t(np.array([40, 7, 0], dtype=np.int32))
     cu = dev_t(np.arange(B + 1, dtype=np.int32))
 
