@@ -4,14 +4,19 @@
 //   x    = the page's new rows (K rotated by position)
 //   s'   = max(max|x| / 127, 2^-126, s if the page holds earlier tokens)
 //   c    = rint(x / s'), and where s' > s the earlier codes c <- rint(c s / s')
-// One workgroup owns a (page, head), keeps the page's new values in registers
-// (32 a thread) between the maximum and the rounding, and so reads each row
-// once.  A page with a value that is not finite gets the scale NaN, which
-// stays while the page fills: what reads the page is NaN.
+// A page with a value that is not finite gets the scale NaN, which stays while
+// the page fills: what reads the page is NaN.
 //
 // Rotation: pair i of position p turns by p * f_i, f_i in turns as 0.64 fixed
-// point, so p * f_i mod 2^64 is the exact fraction of a turn at any position;
-// its upper 32 bits as fp32 are within 2^-26 turns.
+// point, so p * f_i mod 2^64 is the exact fraction of a turn at any position.
+//
+// Both kernels read each row once and keep its values in registers between the
+// maximum and the rounding.
+//   append_pages_kernel: one workgroup per page, K or V, and group of heads;
+//     32 values a thread.  A thread keeps its place in the page from head to
+//     head, so it forms its sines and cosines once for all the heads (K's and
+//     the queries') of its group.
+//   append_token_kernel: one token per sequence; a wave per row.
 #include "common.h"
 #include "kernels.h"
 #include "kvq8.h"
@@ -21,60 +26,50 @@ namespace kvq8 {
 
 namespace {
 
-constexpr int kUnits = 4;  // 8-value units per thread: one page of one head per workgroup
+// cos and sin of 2 pi (pos * freq): the fraction of a turn to 32 bits, taken to
+// the nearest quarter (exact), the rest |x| <= pi / 4 by the Taylor sums
+// (x^11 / 11! and x^10 / 10! under 2.5e-8 there).
+__device__ __forceinline__ void turn(uint64_t freq, int pos, float& c, float& s) {
+    const int t = (int)((uint64_t)(int64_t)pos * freq >> 32);
+    const unsigned quarter = ((unsigned)t + 0x20000000u) >> 30;
+    const float x = (float)(int)((unsigned)t - (quarter << 30)) * (6.28318530717958647692f * 0x1p-32f);
+    const float z = x * x;
+    float a = fmaf(z, 1.f / 362880.f, -1.f / 5040.f);
+    a = fmaf(z, a, 1.f / 120.f);
+    a = fmaf(z, a, -1.f / 6.f);
+    const float sn = fmaf(x * z, a, x);
+    float b = fmaf(z, 1.f / 40320.f, -1.f / 720.f);
+    b = fmaf(z, b, 1.f / 24.f);
+    b = fmaf(z, b, -0.5f);
+    const float cn = fmaf(z, b, 1.f);
+    const float c0 = quarter & 1 ? sn : cn, s0 = quarter & 1 ? cn : sn;
+    c = (quarter + 1) & 2 ? -c0 : c0;
+    s = quarter & 2 ? -s0 : s0;
+}
 
 template <class T>
-__device__ __forceinline__ float to_f32(T x) {
-    return (float)x;
-}
+struct Vec;
+template <>
+struct Vec<float> {
+    typedef float v4 __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Vec<__bf16> {
+    typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+};
 
-__device__ __forceinline__ float2 sincos_turns(uint64_t freq, int pos) {
-    const int t = (int)((uint64_t)(int64_t)pos * freq >> 32);  // fraction of a turn, signed, 2^-32
-    float s, c;
-    sincospif((float)t * 0x1p-31f, &s, &c);
-    return float2{c, s};
-}
-
-// Row d of a rotated row x (8 consecutive head dims from d0).  cs: (cos, sin)
-// of the row's position per pair.
 template <class T>
-__device__ __forceinline__ void rotated8(const T* x, int d0, const AppendArgs& a, const float2* cs, float* y) {
-    float own[8];
+__device__ __forceinline__ void load4(const T* p, float* x) {
+    const typename Vec<T>::v4 v = *reinterpret_cast<const typename Vec<T>::v4*>(p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) own[j] = to_f32(x[d0 + j]);
-    const int half = a.rot >> 1;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int d = d0 + j;
-        y[j] = own[j];
-        if (d < a.rot) {
-            const bool second = a.interleaved ? (d & 1) : d >= half;
-            const int i = a.interleaved ? d >> 1 : second ? d - half : d;
-            const float other = a.interleaved ? own[j ^ 1] : to_f32(x[second ? d - half : d + half]);
-            const float2 w = cs[i];
-            y[j] = second ? fmaf(own[j], w.x, other * w.y) : fmaf(own[j], w.x, -(other * w.y));
-        }
-    }
+    for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
 }
-
-__device__ __forceinline__ unsigned block_max(unsigned x, unsigned* red) {
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float* x) {
+    typename Vec<T>::v4 v;
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, m));
-    const int wave = threadIdx.x >> 6, waves = (blockDim.x + 63) >> 6;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[wave] = x;
-    __syncthreads();
-    for (int w = 0; w < waves; ++w) x = max(x, red[w]);
-    return x;
-}
-
-// Scale of a page from max|x| of its new rows (as bits: NaN above infinity
-// above every number) and the scale of its earlier tokens.
-__device__ __forceinline__ float page_scale(unsigned amax_bits, bool has_old, float old) {
-    if (amax_bits >= 0x7f800000u) return __builtin_nanf("");
-    const float s = fmaxf(__uint_as_float(amax_bits) / 127.f, kMinScale);
-    if (!has_old) return s;
-    return old > s || old != old ? old : s;
+    for (int j = 0; j < 4; ++j) v[j] = (T)x[j];
+    *reinterpret_cast<typename Vec<T>::v4*>(p) = v;
 }
 
 // rint(x * inv) + 128 as a byte: 2^23 * 1.5 + 128 leaves the whole number in
@@ -82,228 +77,442 @@ __device__ __forceinline__ float page_scale(unsigned amax_bits, bool has_old, fl
 __device__ __forceinline__ unsigned code_of(float x, float inv) {
     return __float_as_uint(fmaf(x, inv, 12583040.f)) & 0xffu;
 }
-// An earlier code in the page's new, larger step (r = old / new scale).
-__device__ __forceinline__ unsigned recode(unsigned u, float r) { return code_of((float)((int)u - 128), r); }
+__device__ __forceinline__ unsigned codes4(const float* x, float inv) {
+    return code_of(x[0], inv) | code_of(x[1], inv) << 8 | code_of(x[2], inv) << 16 | code_of(x[3], inv) << 24;
+}
+// Earlier codes in the page's new, larger step (r = old / new scale).
+__device__ __forceinline__ unsigned recode4(unsigned w, float r) {
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = (float)((int)(w >> (8 * k) & 0xffu) - 128);
+    return codes4(x, r);
+}
 
-template <class T>
-__device__ void append_page(const Cache& c, const AppendArgs& a, int b, int j, int h, bool is_v, float2* cs,
-                            unsigned* red) {
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Scale of a page from max|x| of its new rows (as bits: NaN above infinity
+// above every number) and the scale of its earlier tokens.
+struct Scale {
+    float scale, inv, r;
+    bool grown;  // the earlier codes have to be rounded again, times r
+    __device__ __forceinline__ Scale(unsigned amax, bool has_old, float old) {
+        scale = amax >= 0x7f800000u ? __builtin_nanf("") : fmaxf(__uint_as_float(amax) / 127.f, kMinScale);
+        if (has_old && (old > scale || old != old)) scale = old;
+        inv = 1.0f / scale;
+        grown = has_old && old == old && scale != old;
+        r = old / scale;
+    }
+};
+
+__device__ __forceinline__ unsigned wave_umax(unsigned x) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, m));
+    return x;
+}
+
+// Rounds the codes of tokens [0, n) of a page again; one of nt threads.
+__device__ void recode_page(uint8_t* codes, bool is_v, int n, int D, float r, int tid, int nt) {
+    if (!is_v) {
+        for (int i = tid; i < n * D / 16; i += nt) {
+            uint4* p = reinterpret_cast<uint4*>(codes) + i;
+            uint4 w = *p;
+            *p = uint4{recode4(w.x, r), recode4(w.y, r), recode4(w.z, r), recode4(w.w, r)};
+        }
+        return;
+    }
+    // 8 bytes: tokens t .. t + 3 and t + 16 .. t + 19 of one head dim
+    for (int i = tid; i < (n + 31) / 32 * (4 * D); i += nt) {
+        const int t = i / (4 * D) * 32 + (i >> 5 & 3) * 4;
+        uint2* p = reinterpret_cast<uint2*>(codes) + i;
+        uint2 w = *p;
+        const uint2 x = {recode4(w.x, r), recode4(w.y, r)};
+        // bytes of tokens below n
+        const int a = min(max(n - t, 0), 4), b = min(max(n - t - 16, 0), 4);
+        const unsigned ma = a == 4 ? ~0u : (1u << 8 * a) - 1u, mb = b == 4 ? ~0u : (1u << 8 * b) - 1u;
+        *p = uint2{(x.x & ma) | (w.x & ~ma), (x.y & mb) | (w.y & ~mb)};
+    }
+}
+
+// 16 values of a row: head dims dim(j), j = 0 .. 15, of which j and j + 8 (or,
+// interleaved, 2i and 2i + 1) are a rotated pair.  Where the pairs lie rot / 2
+// apart and that is no multiple of 8 (ODD), groups hold what is left over and
+// head dims are taken one by one.
+template <bool ODD>
+struct Group {
+    int d0, d1;   // first head dim of j < 8 and of j >= 8
+    int n0, n1;   // valid ones of each (ODD)
+    int pair;     // first pair, or -1
+    __device__ __forceinline__ void init(int g, int D, const AppendArgs& a) {
+        n0 = n1 = 8;
+        pair = -1;
+        const int half = a.rot >> 1;
+        if (a.rot == 0 || a.interleaved) {
+            d0 = 16 * g;
+            d1 = d0 + 8;
+            if (a.rot) pair = 8 * g;
+        } else {
+            const int ng = (half + 7) >> 3;
+            if (g < ng) {
+                pair = d0 = 8 * g;
+                d1 = d0 + half;
+                if (ODD) n0 = n1 = min(8, half - d0);
+            } else {
+                d0 = a.rot + 16 * (g - ng);
+                d1 = d0 + 8;
+                if (ODD) {
+                    n0 = min(8, max(0, D - d0));
+                    n1 = min(8, max(0, D - d1));
+                }
+            }
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ void load(const T* row, float* x) const {
+        if constexpr (ODD) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = j < n0 ? (float)row[d0 + j] : 0.f;
+                x[8 + j] = j < n1 ? (float)row[d1 + j] : 0.f;
+            }
+        } else {
+            load4(row + d0, x);
+            load4(row + d0 + 4, x + 4);
+            load4(row + d1, x + 8);
+            load4(row + d1 + 4, x + 12);
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ void store(T* row, const float* x) const {
+        if constexpr (ODD) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j < n0) row[d0 + j] = (T)x[j];
+                if (j < n1) row[d1 + j] = (T)x[8 + j];
+            }
+        } else {
+            store4(row + d0, x);
+            store4(row + d0 + 4, x + 4);
+            store4(row + d1, x + 8);
+            store4(row + d1 + 4, x + 12);
+        }
+    }
+    __device__ __forceinline__ void store_codes(uint8_t* row, const float* x, float inv) const {
+        if constexpr (ODD) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j < n0) row[d0 + j] = (uint8_t)code_of(x[j], inv);
+                if (j < n1) row[d1 + j] = (uint8_t)code_of(x[8 + j], inv);
+            }
+        } else {
+            *reinterpret_cast<uint2*>(row + d0) = uint2{codes4(x, inv), codes4(x + 4, inv)};
+            *reinterpret_cast<uint2*>(row + d1) = uint2{codes4(x + 8, inv), codes4(x + 12, inv)};
+        }
+    }
+    __device__ __forceinline__ void angles(const AppendArgs& a, int pos, float* c, float* s) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            c[j] = 1.f;
+            s[j] = 0.f;
+            if (pair >= 0 && pair + j < (a.rot >> 1)) turn(a.freqs[pair + j], pos, c[j], s[j]);
+        }
+    }
+    __device__ __forceinline__ void rotate(const AppendArgs& a, float* x, const float* c, const float* s) const {
+        if (pair < 0) return;
+        const int n = (a.rot >> 1) - pair;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // pair j: (j, j + 8) or (2j, 2j + 1)
+            float& p = a.interleaved ? x[2 * j] : x[j];
+            float& q = a.interleaved ? x[2 * j + 1] : x[j + 8];
+            const float p0 = p, q0 = q;
+            p = j < n ? fmaf(p0, c[j], -(q0 * s[j])) : p0;
+            q = j < n ? fmaf(q0, c[j], p0 * s[j]) : q0;
+        }
+    }
+};
+
+// Grid: (page slots of each sequence) x (head groups) x (K, V).  Threads:
+// page_size * D / 32.
+template <class T, int D, bool ODD>
+__global__ __launch_bounds__(4 * D) void append_pages_kernel(Cache c, AppendArgs a, int page_slots, int groups) {
+    constexpr int U = ODD ? 3 : 2;  // groups of 16 values per thread
+    __shared__ unsigned red[2][16];
+    const int tid = threadIdx.x, nt = blockDim.x, waves = (nt + 63) >> 6;
+    int id = blockIdx.x;
+    const int hg = id % groups;
+    id /= groups;
+    const bool is_v = id & 1;
+    id >>= 1;
+    const int b = id / page_slots, slot = id % page_slots;
     const Seq s = sequence(c, b);
-    if (s.n == 0 || s.bad || s.len == 0) return;
-    const int ps = 1 << c.lps, D = c.D, first = s.len - s.n;
-    const int base = ((first >> c.lps) + j) << c.lps;  // position of the page's first token
-    if (base >= s.len) return;
-    const int page = page_of(c, b, base);
+    if (s.n == 0) return;
+    const int ps = 1 << c.lps;
+    const bool store = !s.bad && s.len > 0;
+    const int first = store ? s.len - s.n : 0;               // a bad sequence's rows count from 0
+    const int base = ((first >> c.lps) + slot) << c.lps;     // position of the page's first token
+    if (base >= first + s.n) return;
+    const int t0 = max(first - base, 0), t1 = min(first + s.n - base, ps);  // the page's new tokens
+    const int64_t row0 = (int64_t)s.row0 + base - first;     // buffer row of page token 0 (may be < 0)
+    const int page = store ? page_of(c, b, base) : -1;
+    const int hn = (c.H + groups - 1) / groups, h0 = hg * hn, h1 = page < 0 ? h0 : min(c.H, h0 + hn);
+    int turns = 0;  // heads done, for the two reduction buffers
+    auto block_max = [&](unsigned x) {
+        unsigned* r = red[turns++ & 1];
+        x = wave_umax(x);
+        if ((tid & 63) == 0) r[tid >> 6] = x;
+        __syncthreads();
+        for (int w = 0; w < waves; ++w) x = max(x, r[w]);
+        return x;
+    };
+
+    if (is_v) {
+        // thread: 8 tokens (4q .. and 16 + 4q ..) of 4 head dims
+        const int unit = tid;
+        const int c4 = unit >> 1 & 3, e = unit & 1, q = unit >> 3 & 3;
+        const int db = unit / 32 % (D / 32), tile = unit / D;
+        const int d0 = db * 32 + e * 16 + c4 * 4, lo = tile * 32 + q * 4;
+        int fresh = 0;  // bit k: token lo + 16 (k / 4) + k % 4 is new
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int tok = lo + (k >> 2) * 16 + (k & 3);
+            fresh |= (tok >= t0 && tok < t1) << k;
+        }
+        float x[8][4], nx[8][4];
+        auto load = [&](int h, float (*to)[4]) {
+            const T* v = static_cast<const T*>(a.v) + h * a.v_hs + d0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (fresh >> k & 1)
+                    load4(v + (row0 + lo + (k >> 2) * 16 + (k & 3)) * a.v_ts, to[k]);
+                else
+                    to[k][0] = to[k][1] = to[k][2] = to[k][3] = 0.f;
+            }
+        };
+        if (h0 < h1) load(h0, x);
+        for (int h = h0; h < h1; ++h) {
+            if (h + 1 < h1) load(h + 1, nx);
+            uint8_t* codes = c.v + page * c.page_stride + h * c.head_stride;
+            float* sp = c.vs + page * c.s_page_stride + h * c.s_head_stride;
+            const float old = t0 > 0 ? *sp : 0.f;
+            unsigned amax = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) amax = max(amax, abs_bits(x[k][j]));
+            const Scale sc(block_max(amax), t0 > 0, old);
+            if (sc.grown) {
+                recode_page(codes, true, t0, D, sc.r, tid, nt);
+                __syncthreads();  // before the new tokens' bytes beside them
+            }
+            if (fresh) {
+                uint2* at = reinterpret_cast<uint2*>(codes + v_byte(lo, d0, D));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint2 w = {0u, 0u}, m = {0u, 0u};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        unsigned& word = k < 4 ? w.x : w.y;
+                        unsigned& mask = k < 4 ? m.x : m.y;
+                        word |= code_of(x[k][j], sc.inv) << 8 * (k & 3);
+                        if (fresh >> k & 1) mask |= 0xffu << 8 * (k & 3);
+                    }
+                    if (fresh != 0xff) {
+                        const uint2 had = at[2 * j];
+                        w.x = (w.x & m.x) | (had.x & ~m.x);
+                        w.y = (w.y & m.y) | (had.y & ~m.y);
+                    }
+                    at[2 * j] = w;
+                }
+            }
+            if (tid == 0) *sp = sc.scale;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[k][j] = nx[k][j];
+        }
+        return;
+    }
+
+    const int half = a.rot >> 1;
+    const int per_row = ODD ? ((half + 7) >> 3) + ((D - a.rot + 15) >> 4) : D / 16;
+    Group<ODD> gr[U];
+    int tok[U];
+    bool live[U];
+    float cs[U][8], sn[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int g = tid + u * nt;
+        tok[u] = g / per_row;
+        live[u] = tok[u] >= t0 && tok[u] < t1;
+        gr[u].init(g % per_row, D, a);
+        if (live[u] && a.freqs) gr[u].angles(a, base + tok[u], cs[u], sn[u]);
+    }
+    for (int h = h0; h < h1; ++h) {
+        uint8_t* codes = c.k + page * c.page_stride + h * c.head_stride;
+        float* sp = c.ks + page * c.s_page_stride + h * c.s_head_stride;
+        const float old = t0 > 0 ? *sp : 0.f;
+        float x[U][16];
+        unsigned amax = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) {
+                gr[u].load(static_cast<const T*>(a.k) + (row0 + tok[u]) * a.k_ts + h * a.k_hs, x[u]);
+                if (a.freqs) gr[u].rotate(a, x[u], cs[u], sn[u]);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) amax = max(amax, abs_bits(x[u][j]));
+            }
+        const Scale sc(block_max(amax), t0 > 0, old);
+        if (sc.grown) recode_page(codes, false, t0, D, sc.r, tid, nt);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) gr[u].store_codes(codes + tok[u] * D, x[u], sc.inv);
+        if (tid == 0) *sp = sc.scale;
+    }
+    if (!a.q) return;
+    const int qn = (a.Hq + groups - 1) / groups, q1 = min(a.Hq, hg * qn + qn);
+    for (int h = hg * qn; h < q1; ++h) {
+        float x[U][16];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) gr[u].load(static_cast<const T*>(a.q) + (row0 + tok[u]) * a.q_ts + h * a.q_hs, x[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) {
+                if (a.freqs) gr[u].rotate(a, x[u], cs[u], sn[u]);
+                if (s.bad) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[u][j] = __builtin_nanf("");
+                }
+                gr[u].store(static_cast<T*>(a.q_out) + (row0 + tok[u]) * a.qo_ts + h * a.qo_hs, x[u]);
+            }
+    }
+}
+
+// One token per sequence: a wave per row (K head, V head or query head), lanes
+// by head dims.  Bound by the latency of length -> page -> scale.
+template <class T, int D>
+__global__ __launch_bounds__(256) void append_token_kernel(Cache c, AppendArgs a) {
+    constexpr int E = D > 64 ? D / 64 : 1;  // head dims per lane: lane + 64 e
+    const int per = 2 * c.H + (a.q ? a.Hq : 0);
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (int64_t)c.B * per) return;
+    const int b = __builtin_amdgcn_readfirstlane((int)(item / per)), x = __builtin_amdgcn_readfirstlane((int)(item % per));
+    const int lane = threadIdx.x & 63;
+    const bool on = D >= 64 || lane < D;
+    const bool is_q = x >= 2 * c.H, is_v = !is_q && x >= c.H;
+    const int h = is_q ? x - 2 * c.H : is_v ? x - c.H : x;
+    const Seq s = sequence(c, b);
+    if (s.n == 0 || (!is_q && (s.bad || s.len == 0))) return;
+    const T* row = is_q   ? static_cast<const T*>(a.q) + s.row0 * a.q_ts + h * a.q_hs
+                   : is_v ? static_cast<const T*>(a.v) + s.row0 * a.v_ts + h * a.v_hs
+                          : static_cast<const T*>(a.k) + s.row0 * a.k_ts + h * a.k_hs;
+    const int pos = s.bad || s.len == 0 ? 0 : s.len - 1;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = on ? (float)row[lane + 64 * e] : 0.f;
+    if (a.freqs && !is_v) {
+        const int half = a.rot >> 1;
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int d = lane + 64 * e;
+            y[e] = v[e];
+            if (d < a.rot) {
+                const bool second = a.interleaved ? d & 1 : d >= half;
+                const float other = (float)row[a.interleaved ? d ^ 1 : second ? d - half : d + half];
+                float cs, sn;
+                turn(a.freqs[a.interleaved ? d >> 1 : second ? d - half : d], pos, cs, sn);
+                y[e] = fmaf(v[e], cs, second ? other * sn : -(other * sn));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = y[e];
+    }
+    if (is_q) {  // all lanes have read their pairs: q_out may be q
+        T* out = static_cast<T*>(a.q_out) + s.row0 * a.qo_ts + h * a.qo_hs;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (on) out[lane + 64 * e] = (T)(s.bad ? __builtin_nanf("") : v[e]);
+        return;
+    }
+    const int page = page_of(c, b, pos);
     if (page < 0) return;
-    const int t0 = max(first - base, 0), t1 = min(s.len - base, ps);  // the page's new tokens
-    const int row0 = s.row0 + base - first;                           // buffer row of page token 0 (may be < 0)
+    const int tok = pos & ((1 << c.lps) - 1);
     uint8_t* codes = (is_v ? c.v : c.k) + page * c.page_stride + h * c.head_stride;
     float* sp = (is_v ? c.vs : c.ks) + page * c.s_page_stride + h * c.s_head_stride;
-    const T* x = is_v ? static_cast<const T*>(a.v) + h * a.v_hs : static_cast<const T*>(a.k) + h * a.k_hs;
-    const int64_t ts = is_v ? a.v_ts : a.k_ts;
-    const float old = t0 > 0 ? *sp : 0.f;
-
-    const int nt = blockDim.x, tid = threadIdx.x;
-    const int units = ps * D / 8;
-    float val[kUnits][8];
+    const float old = tok > 0 ? *sp : 0.f;
     unsigned amax = 0;
-    if (is_v) {
-        // unit (tile, q, d): tokens 32 tile + 4q..+3 and +16
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int id = tid + u * nt;
-            if (id >= units) break;
-            const int d = id % D, tq = id / D;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int tok = (tq >> 2) * 32 + (k >> 2) * 16 + (tq & 3) * 4 + (k & 3);
-                val[u][k] = tok >= t0 && tok < t1 ? to_f32(x[(row0 + tok) * ts + d]) : 0.f;
-                amax = max(amax, __float_as_uint(val[u][k]) & 0x7fffffffu);
-            }
-        }
-    } else {
-        // unit (token, 8 head dims), 32 tokens at a time for the table of angles
-        const int pairs = a.freqs ? a.rot >> 1 : 0, upr = D / 8, per = 32 * upr;  // units per 32 tokens
-        int u = 0;
-#pragma unroll
-        for (int u0 = 0; u0 < kUnits; ++u0)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) val[u0][k] = 0.f;
-        for (int sub = 0; sub < ps; sub += 32) {
-            const int s0 = max(sub, t0), s1 = min(sub + 32, t1);
-            if (pairs && s0 < s1) {
-                __syncthreads();
-                for (int i = tid; i < (s1 - s0) * pairs; i += nt) {
-                    const int tok = s0 + i / pairs, p = i % pairs;
-                    cs[(tok - sub) * pairs + p] = sincos_turns(a.freqs[p], base + tok);
-                }
-                __syncthreads();
-            }
-#pragma unroll
-            for (int u0 = 0; u0 < kUnits; ++u0) {
-                const int id = tid + u0 * nt;
-                const int tok = id / upr;
-                if (id < sub * upr || id >= sub * upr + per) continue;
-                if (tok >= t0 && tok < t1) {
-                    const T* row = x + (row0 + tok) * ts;
-                    const int d0 = (id % upr) * 8;
-                    if (pairs) {
-                        rotated8(row, d0, a, cs + (tok - sub) * pairs, val[u0]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) val[u0][k] = to_f32(row[d0 + k]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) amax = max(amax, __float_as_uint(val[u0][k]) & 0x7fffffffu);
-                }
-            }
-        }
-        (void)u;
+    for (int e = 0; e < E; ++e) amax = max(amax, abs_bits(v[e]));
+    const Scale sc(wave_umax(amax), tok > 0, old);
+    if (sc.grown) {
+        recode_page(codes, is_v, tok, D, sc.r, lane, 64);
+        __threadfence_block();  // before the new token's bytes beside them
     }
-    amax = block_max(amax, red);
-    const float scale = page_scale(amax, t0 > 0, old);
-    const float inv = 1.0f / scale;
-    const bool grown = t0 > 0 && scale != old && old == old;
-    const float r = old / scale;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-        const int id = tid + u * nt;
-        if (id >= units) break;
-        uint2 w = {0u, 0u};
-        if (is_v) {
-            const int d = id % D, tq = id / D;
-            const int lo = (tq >> 2) * 32 + (tq & 3) * 4;  // tokens lo..lo+3 and lo+16..lo+19
-            uint2* at = reinterpret_cast<uint2*>(codes + v_byte(lo, d, D));
-            int fresh = 0, earlier = 0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int tok = lo + (k >> 2) * 16 + (k & 3);
-                fresh += tok >= t0 && tok < t1;
-                earlier += tok < t0;
-            }
-            if (fresh == 0 && !(grown && earlier)) continue;
-            if (fresh < 8) w = *at;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int tok = lo + (k >> 2) * 16 + (k & 3);
-                unsigned& word = k < 4 ? w.x : w.y;
-                const int sh = 8 * (k & 3);
-                if (tok >= t0 && tok < t1)
-                    word = (word & ~(0xffu << sh)) | code_of(val[u][k], inv) << sh;
-                else if (grown && tok < t0)
-                    word = (word & ~(0xffu << sh)) | recode((word >> sh) & 0xffu, r) << sh;
-            }
-            *at = w;
-        } else {
-            const int upr = D / 8, tok = id / upr, d0 = (id % upr) * 8;
-            uint2* at = reinterpret_cast<uint2*>(codes + k_byte(tok, d0, D));
-            const bool fresh = tok >= t0 && tok < t1;
-            if (!fresh && !(grown && tok < t0)) continue;
-            if (!fresh) w = *at;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                unsigned& word = k < 4 ? w.x : w.y;
-                const int sh = 8 * (k & 3);
-                const unsigned n = fresh ? code_of(val[u][k], inv) : recode((word >> sh) & 0xffu, r);
-                word = (word & ~(0xffu << sh)) | n << sh;
-            }
-            *at = w;
-        }
+    for (int e = 0; e < E; ++e) {
+        const int d = lane + 64 * e;
+        if (on) codes[is_v ? v_byte(tok, d, D) : k_byte(tok, d, D)] = (uint8_t)code_of(v[e], sc.inv);
     }
-    if (tid == 0) *sp = scale;
+    if (lane == 0) *sp = sc.scale;
 }
 
-// Queries: one pair (or one head dim past the rotated ones) per thread and
-// step, read and written by the same thread, so q_out may be q.
-template <class T>
-__device__ void rotate_queries(const Cache& c, const AppendArgs& a, int b, int chunk, float2* cs) {
-    const Seq s = sequence(c, b);
-    const int i0 = chunk * 32, i1 = min(s.n, i0 + 32);
-    if (i0 >= i1) return;
-    const int pairs = a.freqs ? a.rot >> 1 : 0, nt = blockDim.x, tid = threadIdx.x;
-    for (int i = tid; i < (i1 - i0) * pairs; i += nt)
-        cs[i] = sincos_turns(a.freqs[i % pairs], max(s.len - s.n, 0) + i0 + i / pairs);
-    __syncthreads();
-    const int items = c.D - pairs;  // pairs, then the head dims that stay
-    const int per_tok = items * a.Hq;
-    const float bad = s.bad ? __builtin_nanf("") : 0.f;
-    for (int i = tid; i < (i1 - i0) * per_tok; i += nt) {
-        const int tok = i / per_tok, rest = i % per_tok, h = rest / items, p = rest % items;
-        const T* x = static_cast<const T*>(a.q) + (s.row0 + i0 + tok) * a.q_ts + h * a.q_hs;
-        T* y = static_cast<T*>(a.q_out) + (s.row0 + i0 + tok) * a.qo_ts + h * a.qo_hs;
-        if (p < pairs) {
-            const int d0 = a.interleaved ? 2 * p : p, d1 = a.interleaved ? d0 + 1 : p + pairs;
-            const float x0 = to_f32(x[d0]), x1 = to_f32(x[d1]);
-            const float2 w = cs[tok * pairs + p];
-            y[d0] = (T)(fmaf(x0, w.x, -(x1 * w.y)) + bad);
-            y[d1] = (T)(fmaf(x1, w.x, x0 * w.y) + bad);
-        } else {
-            y[p + pairs] = (T)(to_f32(x[p + pairs]) + bad);
-        }
-    }
-}
-
-template <class T>
-__global__ __launch_bounds__(1024) void append_kernel(Cache c, AppendArgs a, int page_slots, int q_chunks) {
-    extern __shared__ float2 cs[];  // [32][rot / 2] cos, sin
-    __shared__ unsigned red[16];
-    int id = blockIdx.x;
-    const int kv = c.B * page_slots * c.H * 2;
-    if (id < kv) {
-        const int h = id % c.H;
-        id /= c.H;
-        const bool is_v = id & 1;
-        id >>= 1;
-        append_page<T>(c, a, id / page_slots, id % page_slots, h, is_v, cs, red);
-    } else {
-        id -= kv;
-        rotate_queries<T>(c, a, id / q_chunks, id % q_chunks, cs);
-    }
-}
-
-template <class T>
-__global__ __launch_bounds__(256) void read_kernel(Cache c, ReadArgs a, int tiles) {
+// One 32-token tile of one head: D threads with 8 tokens of 4 head dims of V,
+// D threads with two 16-byte pieces of K rows.
+template <class T, int D>
+__global__ __launch_bounds__(2 * D) void read_kernel(Cache c, ReadArgs a, int tiles) {
     int id = blockIdx.x;
     const int h = id % c.H;
     id /= c.H;
     const int b = id / tiles, tile = id % tiles;
     const Seq s = sequence(c, b);
-    const int first = s.len - s.n, D = c.D, tid = threadIdx.x;
-    if (s.bad) {
-        for (int i = tid; i < 32 * D; i += 256) {
-            const int row = tile * 32 + i / D;
-            if (row >= s.n) continue;
-            static_cast<T*>(a.k)[(s.row0 + row) * a.k_ts + h * a.k_hs + i % D] = (T)__builtin_nanf("");
-            static_cast<T*>(a.v)[(s.row0 + row) * a.v_ts + h * a.v_hs + i % D] = (T)__builtin_nanf("");
-        }
-        return;
-    }
+    const int tid = threadIdx.x;
+    if (s.n == 0 || (s.len == 0 && !s.bad)) return;
+    const int first = s.bad ? 0 : s.len - s.n;
     const int pos0 = ((first >> 5) + tile) << 5;  // tiles lie in one page
-    if (s.n == 0 || s.len == 0 || pos0 >= s.len) return;
-    const int page = page_of(c, b, pos0);
-    const int64_t at = (page < 0 ? 0 : page) * c.page_stride + h * c.head_stride;
-    const int64_t sat = (page < 0 ? 0 : page) * c.s_page_stride + h * c.s_head_stride;
-    const float ks = page < 0 ? __builtin_nanf("") : c.ks[sat], vs = page < 0 ? __builtin_nanf("") : c.vs[sat];
+    if (pos0 >= first + s.n) return;
+    const int page = s.bad ? -1 : page_of(c, b, pos0);
+    const int64_t at = (int64_t)max(page, 0) * c.page_stride + (int64_t)h * c.head_stride;
+    const int64_t sat = (int64_t)max(page, 0) * c.s_page_stride + (int64_t)h * c.s_head_stride;
     const int tb = pos0 & ((1 << c.lps) - 1);  // first token in the page
     const int64_t row0 = (int64_t)s.row0 + pos0 - first;
-    for (int i = tid; i < 4 * D; i += 256) {
-        const int tok = i / (D / 8), d0 = (i % (D / 8)) * 8;
-        if (pos0 + tok < first || pos0 + tok >= s.len) continue;
-        const uint2 w = *reinterpret_cast<const uint2*>(c.k + at + k_byte(tb + tok, d0, D));
-        T* y = static_cast<T*>(a.k) + (row0 + tok) * a.k_ts + h * a.k_hs + d0;
+    const int lo = max(first - pos0, 0), hi = min(first + s.n - pos0, 32);
+    const bool is_v = tid >= D;
+    const float sc = page < 0 ? __builtin_nanf("") : (is_v ? c.vs : c.ks)[sat];
+    auto value = [&](unsigned w, int k) { return (float)((int)(w >> (8 * k) & 0xffu) - 128) * sc; };
+    if (is_v) {
+        const int u = tid % D;
+        const int e = u & 1, c4 = u >> 1 & 3, q = u >> 3 & 3, db = u >> 5;
+        const int d0 = db * 32 + e * 16 + c4 * 4;
+        const uint2* p = reinterpret_cast<const uint2*>(c.v + at + v_byte(tb + 4 * q, d0, D));
+        uint2 w[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            y[k] = (T)((float)((int)(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xffu) - 128) * ks);
-    }
-    for (int i = tid; i < 4 * D; i += 256) {
-        const int q = i / D, d = i % D;
-        const uint2 w = *reinterpret_cast<const uint2*>(c.v + at + v_byte(tb + 4 * q, d, D));
+        for (int j = 0; j < 4; ++j) w[j] = p[2 * j];
+        T* y = static_cast<T*>(a.v) + h * a.v_hs + d0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int tok = (k >> 2) * 16 + 4 * q + (k & 3);
-            if (pos0 + tok < first || pos0 + tok >= s.len) continue;
-            static_cast<T*>(a.v)[(row0 + tok) * a.v_ts + h * a.v_hs + d] =
-                (T)((float)((int)(((k < 4 ? w.x : w.y) >> (8 * (k & 3))) & 0xffu) - 128) * vs);
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = value(k < 4 ? w[j].x : w[j].y, k & 3);
+            if (tok >= lo && tok < hi) store4(y + (row0 + tok) * a.v_ts, x);
+        }
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int i = tid + u * D, tok = i / (D / 16), d0 = i % (D / 16) * 16;
+        const uint4 w = *reinterpret_cast<const uint4*>(c.k + at + k_byte(tb + tok, d0, D));
+        const unsigned ws[4] = {w.x, w.y, w.z, w.w};
+        T* y = static_cast<T*>(a.k) + (row0 + tok) * a.k_ts + h * a.k_hs + d0;
+        if (tok >= lo && tok < hi) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = value(ws[j], k);
+                store4(y + 4 * j, x);
+            }
         }
     }
 }
@@ -316,6 +525,41 @@ __global__ __launch_bounds__(256) void advance_kernel(int* lens, const int* cu, 
     lens[b] = len > 0x7fffffff ? 0x7fffffff : (int)len;
 }
 
+template <class T, int D>
+hipError_t append_d(const Cache& c, const AppendArgs& a, hipStream_t s) {
+    if (c.max_new == 1) {
+        const int64_t rows = (int64_t)c.B * (2 * (int64_t)c.H + (a.q ? a.Hq : 0));
+        if (rows > 0x7fffffff) return hipErrorInvalidConfiguration;
+        hipLaunchKernelGGL((append_token_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, c, a);
+        return hipGetLastError();
+    }
+    const int ps = 1 << c.lps;
+    const int slots = (c.max_new + ps - 2) / ps + 1;  // pages that max_new tokens can lie in
+    // Heads of a workgroup share their sines and cosines; fewer workgroups than
+    // ~2 per CU and role would leave CUs idle.
+    const int64_t pages = (int64_t)(c.T + ps - 1) / ps + c.B;
+    int per = 4;
+    while (per > 1 && pages * ((c.H + per - 1) / per) < 512) per /= 2;
+    const int groups = (c.H + per - 1) / per;
+    const int64_t grid = (int64_t)c.B * slots * 2 * groups;
+    if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    const dim3 nt(ps * D / 32 < 64 ? 64 : ps * D / 32);  // a whole wave: idle lanes have no token
+    if (a.rot && !a.interleaved && a.rot % 16)
+        hipLaunchKernelGGL((append_pages_kernel<T, D, true>), dim3((unsigned)grid), nt, 0, s, c, a, slots, groups);
+    else
+        hipLaunchKernelGGL((append_pages_kernel<T, D, false>), dim3((unsigned)grid), nt, 0, s, c, a, slots, groups);
+    return hipGetLastError();
+}
+
+template <class T, int D>
+hipError_t read_d(const Cache& c, const ReadArgs& a, hipStream_t s) {
+    const int tiles = (c.max_new + 30) / 32 + 1;
+    const int64_t grid = (int64_t)c.B * tiles * c.H;
+    if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((read_kernel<T, D>), dim3((unsigned)grid), dim3(2 * D), 0, s, c, a, tiles);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 bool supported(int D, int page_size) {
@@ -323,32 +567,25 @@ bool supported(int D, int page_size) {
 }
 
 hipError_t launch_append(const Cache& c, const AppendArgs& a, int dtype, hipStream_t s) {
-    const int ps = 1 << c.lps;
-    const int slots = (c.max_new + ps - 2) / ps + 1;  // pages that max_new tokens can lie in
-    const int chunks = a.q ? (c.max_new + 31) / 32 : 0;
-    const int64_t grid = (int64_t)c.B * slots * c.H * 2 + (int64_t)c.B * chunks;
-    if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
-    int nt = ps * c.D / (8 * kUnits);
-    if (nt < 64) nt = 64;
-    const size_t lds = a.freqs ? (size_t)32 * (a.rot / 2) * sizeof(float2) : 0;
-    if (dtype == kF32)
-        hipLaunchKernelGGL((append_kernel<float>), dim3((unsigned)grid), dim3(nt), lds, s, c, a, slots,
-                           chunks ? chunks : 1);
-    else
-        hipLaunchKernelGGL((append_kernel<__bf16>), dim3((unsigned)grid), dim3(nt), lds, s, c, a, slots,
-                           chunks ? chunks : 1);
-    return hipGetLastError();
+    const bool f = dtype == kF32;
+    switch (c.D) {
+        case 32: return f ? append_d<float, 32>(c, a, s) : append_d<__bf16, 32>(c, a, s);
+        case 64: return f ? append_d<float, 64>(c, a, s) : append_d<__bf16, 64>(c, a, s);
+        case 128: return f ? append_d<float, 128>(c, a, s) : append_d<__bf16, 128>(c, a, s);
+        case 256: return f ? append_d<float, 256>(c, a, s) : append_d<__bf16, 256>(c, a, s);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 hipError_t launch_read(const Cache& c, const ReadArgs& a, int dtype, hipStream_t s) {
-    const int tiles = (c.max_new + 30) / 32 + 1;
-    const int64_t grid = (int64_t)c.B * tiles * c.H;
-    if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
-    if (dtype == kF32)
-        hipLaunchKernelGGL((read_kernel<float>), dim3((unsigned)grid), dim3(256), 0, s, c, a, tiles);
-    else
-        hipLaunchKernelGGL((read_kernel<__bf16>), dim3((unsigned)grid), dim3(256), 0, s, c, a, tiles);
-    return hipGetLastError();
+    const bool f = dtype == kF32;
+    switch (c.D) {
+        case 32: return f ? read_d<float, 32>(c, a, s) : read_d<__bf16, 32>(c, a, s);
+        case 64: return f ? read_d<float, 64>(c, a, s) : read_d<__bf16, 64>(c, a, s);
+        case 128: return f ? read_d<float, 128>(c, a, s) : read_d<__bf16, 128>(c, a, s);
+        case 256: return f ? read_d<float, 256>(c, a, s) : read_d<__bf16, 256>(c, a, s);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 hipError_t launch_advance(int* lens, const int* cu, int B, hipStream_t s) {

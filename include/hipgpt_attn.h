@@ -218,7 +218,8 @@ typedef struct hipgpt_kvq8_cache {
  *                it, attention gives zeros.
  *   max_new:     the most new tokens of any sequence.
  * A sequence with lens[b] < n, more tokens than its table holds, or n >
- * max_new is left as it is and gets NaN rows; so does what reads a page index
+ * max_new is left as it is and gets NaN rows (the first max_new); so does what
+ * reads a page index
  * outside [0, num_pages), which appends skip.  Rows that no sequence names
  * (a cu_new that is not increasing or passes T) are left as they were.  Pages
  * that several sequences hold may be read by all, and appended to by none. */
