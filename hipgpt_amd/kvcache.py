@@ -21,6 +21,7 @@ the host; lengths and page tables are read on the device.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -28,13 +29,21 @@ from . import _lib
 from .attention import _need_cuda, _ptr
 
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+# the stream handle alone: torch.cuda.current_stream() builds an object around it, 2.7 us a call
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dtype(name, t):
-    dt = _TYPES.get(t if isinstance(t, torch.dtype) else t.dtype)
+    dt = _TYPES.get(t.dtype)
     if dt is None:
         raise TypeError(f"{name} must be float32 or bfloat16")
     return dt
+
+
+def _tensor(name, t):
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise ValueError(f"{name} must be a [rows, heads, D] tensor")
+    return t
 
 
 class CacheQ8:
@@ -57,6 +66,7 @@ class CacheQ8:
             raise ValueError("k_scale, v_scale must be [pages, heads] with the same strides")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device, self.heads, self.page_size, self.head_dim = k.device, H, ps, D
+        self.index = k.device.index
         self._c = _lib.KvQ8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                  k.stride(0), k.stride(1), k_scale.stride(0), k_scale.stride(1), P, ps, H, D)
         self._ref = ctypes.byref(self._c)
@@ -109,103 +119,103 @@ def rope_freqs(rot_dim, base=10000.0, device="cuda"):
     return torch.tensor(list(f), dtype=torch.int64, device=device)
 
 
-def _rows(name, t, T, heads, D, dtype, device):
-    """(token, head) strides of a [T, heads, D] tensor with contiguous D."""
+def _rows(name, t, shape, dtype, device):
+    """(token, head) strides of a tensor of that shape with contiguous D."""
     if not isinstance(t, torch.Tensor) or t.device != device:
         raise TypeError(f"{name} must be a tensor on {device}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != (T, heads, D) or t.stride(2) != 1:
-        raise ValueError(f"{name} must be [{T}, {heads}, {D}] with contiguous D")
-    return t.stride(0), t.stride(1)
+    st = t.stride()
+    if t.shape != shape or st[2] != 1:
+        raise ValueError(f"{name} must be {list(shape)} with contiguous D")
+    return st[:2]
 
 
-def _call(cache, batch, name, make, stream, owned):
-    """Calls entry point ``name`` with ``make(stream handle)`` as arguments, on the cache's
-    device.  ``owned``: tensors allocated here, which another stream's kernels use."""
-    if batch.device != cache.device:
-        raise ValueError("cache and batch must be on one device")
-    if torch.cuda.current_device() != cache.device.index:
-        with torch.cuda.device(cache.device):
-            return _call(cache, batch, name, make, stream, owned)
+def _on_device(call):
+    """Runs an entry point of this module with its cache's device current."""
+
+    @functools.wraps(call)
+    def run(cache, batch, *args, **kw):
+        if batch.device != cache.device:
+            raise ValueError("cache and batch must be on one device")
+        if torch.cuda.current_device() != cache.index:
+            with torch.cuda.device(cache.device):
+                return call(cache, batch, *args, **kw)
+        return call(cache, batch, *args, **kw)
+
+    return run
+
+
+def _handle(cache, stream, *owned):
+    """Handle of the stream to launch on.  ``owned``: tensors allocated here, on the current
+    stream, that another stream's kernels will use."""
     if stream is None:
-        handle = torch.cuda.current_stream().cuda_stream
-    else:
-        handle = stream.cuda_stream
-        for t in owned:
+        return _raw_stream(cache.index)
+    for t in owned:
+        if t is not None:
             t.record_stream(stream)
-    rc = getattr(_lib.lib(), name)(*make(handle))
-    if rc != _lib.OK:
-        _lib.check(rc, name)
+    return stream.cuda_stream
 
 
+@_on_device
 def append(cache, batch, q, k, v, freqs=None, interleaved=False, q_out=None, advance=False, stream=None):
     """Rotates and quantises the new tokens into the cache; returns the rotated q.
 
     k, v: [T, heads, D], q: [T, Hq, D] or None, all float32 or all bfloat16; ``freqs``:
     :func:`rope_freqs` of the rotated head dims (None: no rotation); ``q_out`` may be q.
     ``advance`` first raises ``batch.lens`` by the new tokens."""
-    dt = _dtype("k", k)
-    T, D, dev = k.shape[0], cache.head_dim, cache.device
-    ks = _rows("k", k, T, cache.heads, D, k.dtype, dev)
-    vs = _rows("v", v, T, cache.heads, D, k.dtype, dev)
-    Hq, qs, os_, owned = 0, (0, 0), (0, 0), ()
+    _tensor("k", k)
+    dt, dtype, dev = _dtype("k", k), k.dtype, cache.device
+    T, D = k.shape[0], cache.head_dim
+    shape = (T, cache.heads, D)
+    ks = _rows("k", k, shape, dtype, dev)
+    vs = _rows("v", v, shape, dtype, dev)
+    Hq, qs, os_, mine, qp, op = 0, (0, 0), (0, 0), None, 0, 0
     if q is not None:
-        if q.dim() != 3:
-            raise ValueError("q must be [T, Hq, D]")
-        Hq = q.shape[1]
-        qs = _rows("q", q, T, Hq, D, k.dtype, dev)
+        Hq = _tensor("q", q).shape[1]
+        shape = (T, Hq, D)
+        qs = _rows("q", q, shape, dtype, dev)
         if q_out is None:
-            q_out = torch.empty((T, Hq, D), device=dev, dtype=k.dtype)
-            owned = (q_out,)
-        os_ = _rows("q_out", q_out, T, Hq, D, k.dtype, dev)
+            q_out = mine = q.new_empty(shape)
+        os_ = _rows("q_out", q_out, shape, dtype, dev)
+        qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
-    rot = 0
+    rot = fp = 0
     if freqs is not None:
-        if freqs.dtype != torch.int64 or freqs.device != dev or freqs.dim() != 1 or not freqs.is_contiguous():
+        if freqs.dtype is not torch.int64 or freqs.device != dev or freqs.dim() != 1 or not freqs.is_contiguous():
             raise TypeError("freqs must be what rope_freqs gives, on the cache's device")
-        rot = 2 * freqs.numel()
-    _call(cache, batch, "hipgpt_kvq8_append", lambda s: (
-        cache._ref, batch._ref, T, _ptr(q), _ptr(q_out), k.data_ptr(), v.data_ptr(), Hq, *qs, *os_, *ks, *vs,
-        _ptr(freqs), rot, 1 if interleaved else 0, dt, 1 if advance else 0, s), stream, owned)
+        rot, fp = 2 * freqs.numel(), freqs.data_ptr()
+    rc = _lib.lib().hipgpt_kvq8_append(
+        cache._ref, batch._ref, T, qp, op, k.data_ptr(), v.data_ptr(), Hq, *qs, *os_, *ks, *vs, fp, rot,
+        1 if interleaved else 0, dt, 1 if advance else 0, _handle(cache, stream, mine))
+    if rc:
+        _lib.check(rc, "hipgpt_kvq8_append")
     return q_out
 
 
+@_on_device
 def read(cache, batch, T, dtype=torch.float32, k=None, v=None, stream=None):
     """(k, v) [T, heads, D]: the values of each sequence's last ``cu_new[b + 1] -
     cu_new[b]`` tokens, packed in that order (T rows in all)."""
     shape = (T, cache.heads, cache.head_dim)
-    owned = []
+    mine = [None, None]
     if k is None:
-        k = torch.empty(shape, device=cache.device, dtype=dtype)
-        owned.append(k)
+        k = mine[0] = torch.empty(shape, device=cache.device, dtype=dtype if v is None else v.dtype)
     if v is None:
-        v = torch.empty(shape, device=cache.device, dtype=k.dtype)
-        owned.append(v)
-    dt = _dtype("k", k)
-    ks = _rows("k", k, *shape, k.dtype, cache.device)
-    vs = _rows("v", v, *shape, k.dtype, cache.device)
-    _call(cache, batch, "hipgpt_kvq8_read",
-          lambda s: (cache._ref, batch._ref, T, k.data_ptr(), v.data_ptr(), *ks, *vs, dt, s), stream, owned)
+        v = mine[1] = torch.empty(shape, device=cache.device, dtype=k.dtype)
+    ks = _rows("k", k, shape, k.dtype, cache.device)
+    vs = _rows("v", v, shape, k.dtype, cache.device)
+    rc = _lib.lib().hipgpt_kvq8_read(cache._ref, batch._ref, T, k.data_ptr(), v.data_ptr(), *ks, *vs, _dtype("k", k),
+                                     _handle(cache, stream, *mine))
+    if rc:
+        _lib.check(rc, "hipgpt_kvq8_read")
     return k, v
 
 
-def _attention_args(cache, q, out, out_dtype):
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        raise ValueError("q must be a [T, Hq, D] tensor")
-    T, Hq, D = q.shape
-    dt = _dtype("q", q)
-    owned = []
-    if out is None:
-        out = torch.empty((T, Hq, cache.head_dim), device=cache.device, dtype=out_dtype)
-        owned.append(out)
-    qs = _rows("q", q, T, Hq, cache.head_dim, q.dtype, cache.device)
-    os_ = _rows("out", out, T, Hq, cache.head_dim, out.dtype, cache.device)
-    return T, Hq, dt, _dtype("out", out), qs, os_, out, owned
-
-
+@functools.lru_cache(maxsize=4096)
 def default_splits(B, T, max_new, Hq, heads, D, max_len):
+    """The split count that the library picks for these sizes."""
     return int(_lib.lib().hipgpt_attn_kvq8_default_splits(B, T, max_new, Hq, heads, D, max_len))
 
 
@@ -213,19 +223,35 @@ def workspace_bytes(T, max_new, Hq, heads, D, num_splits):
     return int(_lib.lib().hipgpt_attn_kvq8_workspace_bytes(T, max_new, Hq, heads, D, num_splits))
 
 
-def _splits(cache, batch, T, Hq, num_splits, workspace, owned):
-    """(split count, workspace, its bytes) of an attention call."""
-    H, D = cache.heads, cache.head_dim
+def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, workspace, stream):
+    """Both attention entry points; ``rows``: (T,) where the entry point takes it."""
+    T, Hq, _ = q.shape
+    H, D, dev = cache.heads, cache.head_dim, cache.device
+    shape = (T, Hq, D)
+    dt = _dtype("q", q)
+    qs = _rows("q", q, shape, q.dtype, dev)
+    mine = [None, None]
+    if out is None:
+        out = mine[0] = q.new_empty(shape, dtype=out_dtype)
+    os_ = _rows("out", out, shape, out.dtype, dev)
     if num_splits is None:
         num_splits = default_splits(batch.size, T, batch.max_new, Hq, H, D, batch.max_len or batch.capacity(cache))
-    ns = max(1, int(num_splits))
-    if workspace is None and ns > 1:
-        workspace = torch.empty(workspace_bytes(T, batch.max_new, Hq, H, D, ns), device=cache.device,
-                                dtype=torch.uint8)
-        owned.append(workspace)
-    return ns, _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size()
+    ns = int(num_splits)
+    wp = nbytes = 0
+    if ns > 1:
+        if workspace is None:
+            workspace = mine[1] = q.new_empty(workspace_bytes(T, batch.max_new, Hq, H, D, ns), dtype=torch.uint8)
+        wp, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    rc = getattr(_lib.lib(), name)(
+        cache._ref, batch._ref, *rows, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_,
+        -1.0 if scale is None else float(scale), dt, _dtype("out", out), 1 if ns < 1 else ns, wp, nbytes,
+        _handle(cache, stream, *mine))
+    if rc:
+        _lib.check(rc, name)
+    return out
 
 
+@_on_device
 def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
            stream=None):
     """softmax(q k^T * scale) v of q [B, Hq, D] over each sequence's cached tokens.
@@ -234,26 +260,17 @@ def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_s
     ``num_splits`` partitions of the work (default: the library's choice for
     ``batch.max_len``); ``workspace``: caller-owned, :func:`workspace_bytes` (allocated
     here if None)."""
-    B, Hq, dt, odt, qs, os_, out, owned = _attention_args(cache, q, out, out_dtype)
-    if B != batch.size:
+    if _tensor("q", q).shape[0] != batch.size:
         raise ValueError("q must have one row per sequence")
-    ns, ws, nbytes = _splits(cache, batch, B, Hq, num_splits, workspace, owned)
-    sc = -1.0 if scale is None else float(scale)
-    _call(cache, batch, "hipgpt_attn_decode_kvq8",
-          lambda s: (cache._ref, batch._ref, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, ns, ws, nbytes,
-                     s), stream, owned)
-    return out
+    return _attention("hipgpt_attn_decode_kvq8", (), cache, batch, q, out, out_dtype, scale, num_splits, workspace,
+                      stream)
 
 
+@_on_device
 def prefill(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
             stream=None):
     """Causal attention of each sequence's new tokens (q [T, Hq, D], packed as
     ``batch.cu_new``) over its cache, which holds them already.  The rest as
     :func:`decode`."""
-    T, Hq, dt, odt, qs, os_, out, owned = _attention_args(cache, q, out, out_dtype)
-    ns, ws, nbytes = _splits(cache, batch, T, Hq, num_splits, workspace, owned)
-    sc = -1.0 if scale is None else float(scale)
-    _call(cache, batch, "hipgpt_attn_prefill_kvq8",
-          lambda s: (cache._ref, batch._ref, T, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_, sc, dt, odt, ns, ws,
-                     nbytes, s), stream, owned)
-    return out
+    return _attention("hipgpt_attn_prefill_kvq8", (_tensor("q", q).shape[0],), cache, batch, q, out, out_dtype, scale,
+                      num_splits, workspace, stream)
