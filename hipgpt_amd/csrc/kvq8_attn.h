@@ -10,7 +10,21 @@ namespace kvq8 {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 
+// Weights are kept as p * 2^7 relative to a running maximum m that moves only
+// when a tile exceeds it by more than 2^8: fp16 then holds p up to 2^15, down to
+// 2^-31 of the row's largest.
+constexpr float kShift = 7.f;
+constexpr float kLazy = 8.f;
+// V scales under this share of the largest count as this share of it.
+constexpr float kMinRatio = 0x1p-40f;
+
+// k with vs < 2^(k - 126); 0 for NaN
+__device__ __forceinline__ int scale_exp(float vs) {
+    const int k = (int)(__float_as_uint(vs) >> 23);
+    return k < 255 ? k : 0;
+}
 
 // Two codes of word w as fp16 numbers.
 template <int HI>

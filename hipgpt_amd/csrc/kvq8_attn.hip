@@ -12,8 +12,8 @@
 //     [2^13, 2^14): a bf16 q is then one exact term (what is 2^-37 of the
 //     largest element or less rounds), an fp32 q two terms, off by 2^-23 of
 //     each element at most.
-//   * p, kept within 2^15 of the row's running maximum, is one term for a
-//     bf16 result (off by 2^-12 of itself) and two for an fp32 result.
+//   * p, relative to a running maximum of the row, is one term for a bf16
+//     result (off by 2^-12 of itself) and two for an fp32 result.
 // With 16-row tiles the second terms cost nothing: they are columns of their
 // own in the same product (8 rows a tile instead of 16), and the two halves
 // are added once per score and once at the end.
@@ -21,8 +21,9 @@
 // S^T = K Q^T (16 tokens x 16 rows): lane (c, q) of the accumulator holds
 // tokens 4q..4q+3 of row c; two such products make the 32-token B operand of
 // O^T = V^T P^T without leaving registers, the cache's V tiles being in that
-// token order.  V scales are applied to p relative to the largest met so far,
-// one number for all rows, so a page costs one multiplication per score.
+// token order.  A V scale is applied to p relative to a power of two above the
+// largest met so far, in the exponent; the row sum takes it out again once a
+// tile.
 #include "common.h"
 #include "kernels.h"
 #include "kvq8_attn.h"
@@ -32,47 +33,53 @@ namespace kvq8 {
 
 namespace {
 
-constexpr int NW = 4;            // waves per workgroup
-constexpr float kPShift = 15.f;  // p is kept as p * 2^15: fp16 then holds 2^-39 .. 1
+constexpr int NW = 4;  // waves per workgroup
 
 __device__ __forceinline__ float xor8_add(float x) {  // + the lane 8 places away in its row of 16
     const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false);
     return x + __int_as_float(y);
 }
-// over the four lanes that hold one column
+// over the four lanes (16 apart) that hold one column
 __device__ __forceinline__ float col_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float col_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Raw codes of one 32-token tile of one head.
+// Raw codes of one 32-token tile of one head.  Non-temporal: a decode step
+// reads them once (572 MB of 32/8 heads D128: 119 -> 108 us).
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    return uint4{v[0], v[1], v[2], v[3]};
+}
 template <int D>
 struct Tile {
     static constexpr int KL = D / 64 ? D / 64 : 1;  // 16-byte loads of a 16-token K sub-tile (one of 8 bytes at D = 32)
     uint4 k[2][KL];
     uint4 v[D / 32];
-};
-
-template <int D>
-__device__ __forceinline__ void load_tile(Tile<D>& t, const uint8_t* kp, const uint8_t* vp, int c, int q, int lane) {
+    float ks, vs;
+    __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int c, int q, int lane) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        if constexpr (D == 32) {
-            const uint2 w = *reinterpret_cast<const uint2*>(kp + (s * 16 + c) * D + q * 8);
-            t.k[s][0] = uint4{w.x, w.y, 0u, 0u};
-        } else {
+        for (int s = 0; s < 2; ++s) {
+            if constexpr (D == 32) {
+                const uint2 w = *reinterpret_cast<const uint2*>(kp + (s * 16 + c) * D + q * 8);
+                k[s][0] = uint4{w.x, w.y, 0u, 0u};
+            } else {
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i)
-                t.k[s][i] = *reinterpret_cast<const uint4*>(kp + (s * 16 + c) * D + i * 64 + q * 16);
+                for (int i = 0; i < D / 64; ++i) k[s][i] = load16(kp + (s * 16 + c) * D + i * 64 + q * 16);
+            }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) t.v[i] = *reinterpret_cast<const uint4*>(vp + i * 1024 + lane * 16);
-}
+        for (int i = 0; i < D / 32; ++i) v[i] = load16(vp + i * 1024 + lane * 16);
+    }
+};
 
 // First head dim of the 8 that lane quarter q holds in k-step s of Q K^T.
 template <int D>
@@ -84,7 +91,7 @@ __device__ __forceinline__ int q_dim(int s, int q) {
 // its keys; the four waves take every fourth 32-token tile and are joined in
 // LDS.  TERMS: columns per row (2: q and p as two fp16 terms).
 template <int D, int TERMS, class TI, class TO>
-__global__ __launch_bounds__(NW * 64) void attn_rows_kernel(Cache c, AttnArgsQ8 a, int row_blocks) {
+__global__ __launch_bounds__(NW * 64, D <= 64 ? 4 : D == 128 ? 3 : 2) void attn_rows_kernel(Cache c, AttnArgsQ8 a, int row_blocks) {
     constexpr int RPB = 16 / TERMS;  // rows per block
     __shared__ float s_m[NW][16], s_l[NW][16], s_ref[NW];
     __shared__ __attribute__((aligned(16))) float s_o[NW][16][D + 4];
@@ -105,6 +112,7 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_kernel(Cache c, AttnArgsQ8 
     const int first = s.len - s.n;
     const int row = min(r0 + col % RPB, rows - 1);  // columns past the last row repeat it
     const int lim = s.bad ? 0 : first + row / G + 1;  // keys that the row sees
+    const int low = s.bad ? 0 : first + r0 / G + 1;   // ... the block's first row
     const int top = s.bad ? 0 : first + min(r0 + RPB - 1, rows - 1) / G + 1;
     const int tiles_all = (top + kTile - 1) / kTile;
     const int per = (tiles_all + a.nsplit - 1) / a.nsplit;
@@ -137,19 +145,26 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_kernel(Cache c, AttnArgsQ8 
     floatx4 o[D / 16];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float m = kMaxInit, l = 0.f, ref = 0.f;
+    float m = kMaxInit, l = 0.f;
+    int kref = 0;
 
+    // Two tiles' codes in registers (D <= 128): while one is multiplied the
+    // wave's next is on its way.
     TileMeta meta;
+    Tile<D> tl[2];
     int cnt = 0;
-    for (int t = tile0 + wave; t < tile1; t += NW, ++cnt) {
+    auto fetch = [&](Tile<D>& to, int t) {
         if ((cnt & 63) == 0) meta.load(c, b, h, t, NW, tile1, lane);
         const int page = __builtin_amdgcn_readlane(meta.page, cnt & 63);
-        const float ks = lane_value(meta.ks, cnt & 63), vs = lane_value(meta.vs, cnt & 63);
-        const int tok = (t * kTile) & ((1 << c.lps) - 1);
-        const int64_t at = (int64_t)page * c.page_stride + (int64_t)h * c.head_stride + tok * D;
-        Tile<D> tl;
-        load_tile<D>(tl, c.k + at, c.v + at, col, q4, lane);
-
+        to.ks = lane_value(meta.ks, cnt & 63);
+        to.vs = lane_value(meta.vs, cnt & 63);
+        ++cnt;
+        const int64_t at = (int64_t)page * c.page_stride + (int64_t)h * c.head_stride +
+                           ((t * kTile) & ((1 << c.lps) - 1)) * D;
+        to.load(c.k + at, c.v + at, col, q4, lane);
+    };
+    auto process = [&](const Tile<D>& tl, int t) {
+        const float f = sc * tl.ks, vs_now = tl.vs;
         floatx4 sv[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -161,55 +176,95 @@ __global__ __launch_bounds__(NW * 64) void attn_rows_kernel(Cache c, AttnArgsQ8 
                 sv[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qv[i], sv[u], 0, 0, 0);
             }
         }
-        float f = sc * ks, mt = kMaxInit;
+        const int left = lim - t * kTile - 4 * q4;  // score (u, r) is seen: 16 u + r below this
+        const bool edge = (t + 1) * kTile > low;     // some row does not see some token
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < 4; ++r)
                 if (TERMS == 2) sv[u][r] = xor8_add(sv[u][r]);
-                sv[u][r] = t * kTile + u * 16 + q4 * 4 + r < lim ? sv[u][r] * f : kNegInf;
-                mt = fmaxf(mt, sv[u][r]);
-            }
-        mt = col_max(mt);
-        const float mn = fmaxf(m, mt);
-        float alpha = fast_exp2(m - mn);
-        m = mn;
+        if (edge) {
+            asm volatile("");  // a branch: most tiles have no edge
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (16 * u + r >= left) sv[u][r] = kNegInf;
+        }
+        float mt = sv[0][0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r) mt = fmaxf(mt, sv[r >> 2][r & 3]);
+        mt = col_max(mt) * f;  // NaN (a scale of NaN or 0) moves nothing
+        float alpha = 1.f;
+        if (mt > m + kLazy) {
+            alpha = fast_exp2(m - mt);
+            m = mt;
+        }
         l *= alpha;
-        if (vs > ref) {
-            alpha *= ref / vs;
-            ref = vs;
+        const int k = scale_exp(vs_now);
+        if (k > kref) {
+            alpha = __builtin_amdgcn_ldexpf(alpha, kref - k);
+            kref = k;
         }
         if (__any(alpha != 1.f)) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
         }
-        const float ratio = ref > 0.f ? vs / ref : vs;
+        const float ratio = fmaxf(__builtin_amdgcn_ldexpf(vs_now, 126 - kref), kMinRatio);
+        const float e0 = (kShift - m) + (vs_now == vs_now ? __builtin_amdgcn_logf(ratio) : vs_now);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sv[u][r] = fast_exp2(fmaf(sv[u][r], f, e0));
+        if (edge) {  // also where a scale of 0 or NaN made NaN of what a row does not see
+            asm volatile("");
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (16 * u + r >= left) sv[u][r] = 0.f;
+        }
+        float sum = 0.f;
         half8 pv;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = fast_exp2(sv[u][r] - m + kPShift);
-                l += p;
-                const float w = sv[u][r] == kNegInf ? 0.f : p * ratio;
-                const _Float16 hi = (_Float16)w;
-                pv[u * 4 + r] = TERMS == 2 && col >= 8 ? (_Float16)(w - (float)hi) : hi;
+                sum += sv[u][r];
+                const _Float16 hi = (_Float16)sv[u][r];
+                pv[u * 4 + r] = TERMS == 2 && col >= 8 ? (_Float16)(sv[u][r] - (float)hi) : hi;
             }
+        l = fmaf(sum, __builtin_amdgcn_rcpf(ratio), l);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
             o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(tl.v[i].x, tl.v[i].y), pv, o[2 * i], 0, 0, 0);
             o[2 * i + 1] =
                 __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(tl.v[i].z, tl.v[i].w), pv, o[2 * i + 1], 0, 0, 0);
         }
+    };
+    if constexpr (D <= 128) {
+        if (tile0 + wave < tile1) fetch(tl[0], tile0 + wave);
+        for (int t = tile0 + wave; t < tile1; t += 2 * NW) {
+            if (t + NW < tile1) fetch(tl[1], t + NW);
+            process(tl[0], t);
+            if (t + NW >= tile1) break;
+            if (t + 2 * NW < tile1) fetch(tl[0], t + 2 * NW);
+            process(tl[1], t + NW);
+        }
+    } else {  // no registers for a second tile
+        for (int t = tile0 + wave; t < tile1; t += NW) {
+            fetch(tl[0], t);
+            process(tl[0], t);
+        }
     }
 
-    // join the waves: true O = o * ref, on the common maximum
+    // join the waves: O = o * (V reference), on the common maximum
     l = col_sum(l);
     if (q4 == 0) {
         s_m[wave][col] = m;
         s_l[wave][col] = l;
     }
-    if (lane == 0) s_ref[wave] = ref;
+    if (lane == 0) s_ref[wave] = __builtin_amdgcn_ldexpf(1.f, kref - 126);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) *reinterpret_cast<floatx4*>(&s_o[wave][col][i * 16 + q4 * 4]) = o[i];
     __syncthreads();
@@ -353,8 +408,16 @@ int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int max_len) 
         return blocks < tile_shares(D) && max_len >= 1024 ? tile_shares(D) : 1;
     }
     const int64_t wgs = Hkv * B * ((max_new * G + 15) / 16);
+    // One workgroup per CU at least, none with fewer than 256 keys (the join is
+    // a launch of ~3 us: 1000 keys of 12 heads D64 10.5 us whole, 10.8 in two),
+    // and two per CU where whole rows are so long that the longest of them
+    // decides (64 sequences of 512 .. 8192 keys, 8 heads D128: 113 -> 109 us).
+    // More splits lose: 2 sequences of 131072 and 65537 keys 83 / 83 / 87 / 96 us
+    // at 16 / 32 / 64 / 128.
     int n = 1;
-    while (n < 256 && wgs * n <= 512 && max_len / (2 * n) >= 256) n *= 2;
+    while (n < 256 && max_len / (2 * n) >= 256 && max_len > 1024 &&
+           (wgs * n < 256 || (wgs * n <= 512 && max_len / n >= 8192)))
+        n *= 2;
     return n;
 }
 

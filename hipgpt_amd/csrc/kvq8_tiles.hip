@@ -33,9 +33,6 @@ using fa::halves_sum;
 constexpr int TW = 4;              // waves
 constexpr int ROWS = TW * 32;      // query rows per workgroup
 constexpr int STAGE = 64;          // tokens per LDS buffer
-constexpr float kShift = 7.f;      // p is kept as p * 2^7 ...
-constexpr float kLazy = 8.f;       // ... and exceeds the running maximum by 2^8 at most
-constexpr float kMinRatio = 0x1p-40f;  // V scales under this share of the largest count as this share of it
 
 template <int D>
 struct Stage {
@@ -50,12 +47,6 @@ struct Flight {
     static constexpr int N = D >= 64 ? D / 64 : 1;
     uint4 k[N], v[N];
 };
-
-// k with vs < 2^(k - 126); 0 for NaN
-__device__ __forceinline__ int scale_exp(float vs) {
-    const int k = (int)(__float_as_uint(vs) >> 23);
-    return k < 255 ? k : 0;
-}
 
 __device__ __forceinline__ half8 load_half8(const _Float16* p) { return *reinterpret_cast<const half8*>(p); }
 
@@ -190,6 +181,8 @@ __device__ __forceinline__ void run_piece(const Cache& c, const AttnArgsQ8& a, c
     const int rq = col >> 2;
     const int krow = 4 * (2 * (rq >> 2) + (rq & 1) + 4 * ((rq >> 1) & 1)) + (col & 3);
 
+    float minus_one = -1.f;
+    asm("" : "+s"(minus_one));
     float cur_ks[2] = {0.f, 0.f}, cur_vs[2] = {0.f, 0.f};
     if (stage0 < stage1) {
         load_stage(stage0);
@@ -273,16 +266,27 @@ __device__ __forceinline__ void run_piece(const Cache& c, const AttnArgsQ8& a, c
             half8 pv[TP][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const _Float16 hi = (_Float16)sv[u][r];
-                    pv[0][2 * u + (r >> 3)][r & 7] = hi;
-                    if (TP == 2) pv[TP - 1][2 * u + (r >> 3)][r & 7] = (_Float16)(sv[u][r] - (float)hi);
-                }
                 float sum = fa::kSumInit;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sum += sv[u][r];
                 l = fmaf(sum, __builtin_amdgcn_rcpf(ratio[u]), l);
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float2v x = {sv[u][r], sv[u][r + 1]};
+                    const half2v hi = __builtin_convertvector(x, half2v);
+                    half8& ph = pv[0][2 * u + (r >> 3)];
+                    ph[r & 7] = hi[0];
+                    ph[(r & 7) + 1] = hi[1];
+                    if (TP == 2) {
+                        // what is left: one mixed-precision fma each (minus_one is not a
+                        // constant to the compiler, which would convert and subtract)
+                        const float2v y = {fmaf((float)hi[0], minus_one, x[0]), fmaf((float)hi[1], minus_one, x[1])};
+                        const half2v lo = __builtin_convertvector(y, half2v);
+                        half8& pl = pv[TP - 1][2 * u + (r >> 3)];
+                        pl[r & 7] = lo[0];
+                        pl[(r & 7) + 1] = lo[1];
+                    }
+                }
             }
             const _Float16* vp = now.v + lane * 8;
 #pragma unroll

@@ -171,6 +171,7 @@ def test_attention_refusals():
     assert dec(None, batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 1, None, 0, None) == _lib.ERR_INVALID
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, None, 0, None) == _lib.ERR_WORKSPACE
     wb = L.hipgpt_attn_kvq8_workspace_bytes
+    # parts of every row where few rows share a cached head, else two slots of 128 rows a share
     need = wb(2, 1, 4, 2, 64, 3)
     assert need == 2 * 4 * 3 * 66 * 4
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, P, need - 4, None) == _lib.ERR_WORKSPACE
@@ -178,10 +179,6 @@ def test_attention_refusals():
     assert wb(2, 1, 4, 2, 64, 1) == wb(0, 1, 4, 2, 64, 4) == wb(2, 1, 5, 2, 64, 4) == 0
     assert wb(2, 1, 4, 2, 64, 5000) == wb(2, 1, 4, 2, 64, 1024)
     pre = L.hipgpt_attn_prefill_kvq8
-    # 10 rows of a cached head: split rows; 100: shares of 128-row blocks, two slots each
-    need = wb(7, 5, 4, 2, 64, 2)
-    assert need == 7 * 4 * 2 * 66 * 4
-    assert pre(cache(), batch(), 7, P, P, 4, *s, *s, -1.0, 0, 0, 2, P, need - 4, None) == _lib.ERR_WORKSPACE
     need = wb(70, 50, 4, 2, 64, 3)
     assert need == 3 * (4 + 2 * 128 * (64 + 4)) * 4
     assert pre(cache(), batch(max_new=50), 70, P, P, 4, *s, *s, -1.0, 0, 0, 3, P, need - 4, None) == _lib.ERR_WORKSPACE
@@ -190,7 +187,8 @@ def test_attention_refusals():
     assert ds(0, 2, 1, 4, 4, 64, 99999) == ds(2, 0, 1, 4, 4, 64, 99999) == ds(2, 2, 0, 4, 4, 64, 99999) == 1
     assert ds(1, 1, 1, 8, 8, 64, 100) == 1
     assert 16 <= ds(1, 1, 1, 8, 8, 64, 1 << 17) <= 256
-    assert ds(1, 4096, 4096, 8, 8, 128, 1 << 15) == 512 and ds(64, 65536, 1024, 8, 8, 128, 1024) == 1 == ds(1, 500, 500, 8, 8, 128, 1000)
+    assert ds(1, 4096, 4096, 8, 8, 128, 1 << 15) == 512 and ds(64, 65536, 1024, 8, 8, 128, 1024) == 1
+    assert ds(1, 500, 500, 8, 8, 128, 1000) == 1
 
 
 def test_python_wrappers_refuse_host_tensors():
