@@ -22,6 +22,7 @@ namespace hipgpt {
 namespace kvq8 {
 
 constexpr int kTile = 32;        // tokens per V tile
+constexpr int kMaxLen = 0x7fffff00;  // tokens of a sequence: a tile past it is still an int
 constexpr int kMaxSplits = 1024;  // of the keys, or shares
 // Smallest scale: codes of values under it stay within [-127, 127] and its
 // reciprocal is finite.
@@ -59,7 +60,7 @@ __host__ __device__ inline Seq sequence(const Cache& a, int b) {
     // rows outside the packed buffers: none of them is touched
     s.n = s.row0 >= 0 && end > s.row0 && end <= a.T ? (int)(end - s.row0) : 0;
     s.len = a.lens[b];
-    s.bad = s.n > a.max_new || (s.len < s.n && (a.cu || s.len < 0)) ||
+    s.bad = s.n > a.max_new || (s.len < s.n && (a.cu || s.len < 0)) || s.len > kMaxLen ||
             (int64_t)s.len > ((int64_t)a.max_pages << a.lps);
     if (s.n > a.max_new) s.n = a.max_new;
     return s;

@@ -24,7 +24,8 @@ int problem(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, kvq8:
     if (!c || !b || !c->k || !c->v || !c->k_scale || !c->v_scale || !b->block_table || !b->lens)
         return HIPGPT_ERR_INVALID;
     if (c->num_pages <= 0 || c->heads <= 0 || c->head_dim <= 0 || c->page_size <= 0 || b->batch <= 0 ||
-        b->max_pages <= 0 || b->max_new <= 0 || T <= 0 || b->table_stride < 0 || (b->batch > 1 && b->table_stride == 0))
+        b->max_pages <= 0 || b->max_new <= 0 || T <= 0 || b->table_stride < 0 ||
+        (b->batch > 1 && b->table_stride < b->max_pages))
         return HIPGPT_ERR_INVALID;
     if (!b->cu_new && (b->max_new != 1 || T != b->batch)) return HIPGPT_ERR_INVALID;
     if (!kvq8::supported(c->head_dim, c->page_size)) return HIPGPT_ERR_UNSUPPORTED;
@@ -66,6 +67,7 @@ int attention(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, con
     if (!q || !o || Hq <= 0 || Hq % k.H != 0 || !std::isfinite(scale) || !is_dtype(dtype) || !is_dtype(out_dtype))
         return HIPGPT_ERR_INVALID;
     if (dtype == HIPGPT_F32 && out_dtype == HIPGPT_BF16) return HIPGPT_ERR_UNSUPPORTED;
+    if ((int64_t)k.max_new * (Hq / k.H) > (1 << 30)) return HIPGPT_ERR_UNSUPPORTED;  // rows of one cached head
     if (!rows16(q, q_ts, q_hs, dtype) || !rows16(o, o_ts, o_hs, out_dtype)) return HIPGPT_ERR_UNSUPPORTED;
     const int64_t cap = (int64_t)k.max_pages << k.lps;
     int ns = num_splits > 0 ? num_splits

@@ -12,11 +12,12 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 
-// Weights are kept as p * 2^7 relative to a running maximum m that moves only
-// when a tile exceeds it by more than 2^8: fp16 then holds p up to 2^15, down to
-// 2^-31 of the row's largest.
-constexpr float kShift = 7.f;
-constexpr float kLazy = 8.f;
+// Weights are kept as p * 2^(15 - lazy) relative to a running maximum m that
+// moves only when a tile exceeds it by more than 2^lazy, so that O is seldom
+// scaled again: fp16 then holds p up to 2^15, down to 2^-24 / 2^(15 - lazy) of
+// the row's largest.  An fp32 result (two terms) keeps 4 bits more of the small
+// ones than a bf16 result.
+constexpr float lazy_bits(int terms) { return terms == 2 ? 4.f : 8.f; }
 // V scales under this share of the largest count as this share of it.
 constexpr float kMinRatio = 0x1p-40f;
 

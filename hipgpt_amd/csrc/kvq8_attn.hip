@@ -196,7 +196,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 4 : D == 128 ? 3 : 2) void attn_
         for (int r = 1; r < 8; ++r) mt = fmaxf(mt, sv[r >> 2][r & 3]);
         mt = col_max(mt) * f;  // NaN (a scale of NaN or 0) moves nothing
         float alpha = 1.f;
-        if (mt > m + kLazy) {
+        if (mt > m + lazy_bits(TERMS)) {
             alpha = fast_exp2(m - mt);
             m = mt;
         }
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(NW * 64, D <= 64 ? 4 : D == 128 ? 3 : 2) void attn_
             for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
         }
         const float ratio = fmaxf(__builtin_amdgcn_ldexpf(vs_now, 126 - kref), kMinRatio);
-        const float e0 = (kShift - m) + (vs_now == vs_now ? __builtin_amdgcn_logf(ratio) : vs_now);
+        const float e0 = (15.f - lazy_bits(TERMS) - m) + (vs_now == vs_now ? __builtin_amdgcn_logf(ratio) : vs_now);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll

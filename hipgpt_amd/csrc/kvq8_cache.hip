@@ -520,6 +520,7 @@ __global__ __launch_bounds__(2 * D) void read_kernel(Cache c, ReadArgs a, int ti
 __global__ __launch_bounds__(256) void advance_kernel(int* lens, const int* cu, int B) {
     const int b = blockIdx.x * 256 + threadIdx.x;
     if (b >= B) return;
+    if (lens[b] < 0) return;  // a slot without a sequence
     const int64_t n = cu ? (int64_t)cu[b + 1] - cu[b] : 1;
     const int64_t len = lens[b] + (n > 0 ? n : 0);
     lens[b] = len > 0x7fffffff ? 0x7fffffff : (int)len;

@@ -12,10 +12,8 @@
 //     kq = h + 2 (r / 8) + 4 (r / 4 % 2): registers 8s .. 8s+7 are then the 8
 //     tokens that the cache's V tile keeps together for lane quarter 2s + h,
 //     so that P^T is the B operand of O^T = V^T P^T as it stands.
-//   p = 2^(s - m + 7): the running maximum m moves only when a tile exceeds it
-//     by more than 2^8 (fp16 holds p up to 2^15), and the V scale relative to
-//     the largest met so far rides in the exponent; the row sum takes it out
-//     again once per tile.
+//   The V scale relative to a power of two above the largest met so far rides
+//     in the exponent of p; the row sum takes it out again once per tile.
 #include <type_traits>
 
 #include "common.h"
@@ -232,7 +230,7 @@ __device__ __forceinline__ void run_piece(const Cache& c, const AttnArgsQ8& a, c
             // V scale: a power of two 2^(kref - 126) above every one met is taken out of O
             const int k = max(scale_exp(cur_vs[0]), scale_exp(cur_vs[1]));
             float alpha = 1.f;
-            if (mt > m + kLazy) {
+            if (mt > m + lazy_bits(TP)) {
                 alpha = fast_exp2(m - mt);
                 m = mt;
             }
@@ -250,7 +248,7 @@ __device__ __forceinline__ void run_piece(const Cache& c, const AttnArgsQ8& a, c
             for (int u = 0; u < 2; ++u) {
                 const float vs = cur_vs[u];
                 ratio[u] = fmaxf(__builtin_amdgcn_ldexpf(vs, 126 - kref), kMinRatio);
-                e0[u] = (kShift - m) + (vs == vs ? __builtin_amdgcn_logf(ratio[u]) : vs);
+                e0[u] = (15.f - lazy_bits(TP) - m) + (vs == vs ? __builtin_amdgcn_logf(ratio[u]) : vs);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sv[u][r] = fast_exp2(fmaf(sv[u][r], f[u], e0[u]));
             }

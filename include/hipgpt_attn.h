@@ -213,16 +213,16 @@ typedef struct hipgpt_kvq8_cache {
  *   cu_new:      int [batch + 1]: sequence b's new tokens are rows cu_new[b]
  *                .. cu_new[b + 1] - 1 of the packed buffers and positions
  *                lens[b] - n .. lens[b] - 1.  NULL: one token each, row b
- *                (then T = batch and max_new = 1).
- *                lens[b] = 0 is then an empty slot: appends and reads skip
- *                it, attention gives zeros.
+ *                (then T = batch and max_new = 1).  lens[b] = 0 is then an
+ *                empty slot: appends and reads skip it, attention gives zeros.
  *   max_new:     the most new tokens of any sequence.
- * A sequence with lens[b] < n, more tokens than its table holds, or n >
- * max_new is left as it is and gets NaN rows (the first max_new); so does what
- * reads a page index
+ * A sequence with lens[b] < n (any negative length: a slot without a
+ * sequence), more tokens than its table holds, or n > max_new is left as it is
+ * and gets NaN rows (the first max_new); so does what reads a page index
  * outside [0, num_pages), which appends skip.  Rows that no sequence names
  * (a cu_new that is not increasing or passes T) are left as they were.  Pages
- * that several sequences hold may be read by all, and appended to by none. */
+ * that several sequences hold may be read by all, and appended to by none.
+ * table_stride >= max_pages. */
 typedef struct hipgpt_kvq8_batch {
     const int* block_table;
     int64_t table_stride;
@@ -238,13 +238,15 @@ int hipgpt_rope_freqs(uint64_t* freqs, int rot_dim, double base);
 /* Appends the new tokens' keys and values, rotated by position on the way.
  *   q, k, v: [T] rows of Hq / heads / heads head rows in `dtype`, element
  *            (t, h, d) at X[t * x_ts + h * x_hs + d]; 16-byte aligned rows.
- *   q_out:   receives the rotated q (may be q); q and q_out NULL: none.
+ *   q_out:   receives the rotated q (q itself, or memory apart from q, k and
+ *            v); q and q_out NULL: none.
  *   freqs:   device [rot_dim / 2] as hipgpt_rope_freqs gives them: pair i of
  *            position p turns by p * freqs[i] (exact at any position).  The
  *            pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) where
  *            interleaved; head dims from rot_dim on stay.  NULL: no rotation.
  *   advance: non-zero first raises lens[b] by the sequence's new tokens (the
- *            first layer's append of a step); 0: lens includes them already.
+ *            first layer's append of a step), negative ones apart; 0: lens
+ *            includes them already.
  * Per (page, head) the new scale is max|x| / 127 over the page's new rows, at
  * least 2^-126 and, where the page holds earlier tokens, at least their scale;
  * where that grows, their codes are rounded again to the new one.  Codes are
@@ -280,7 +282,8 @@ int hipgpt_kvq8_read(const hipgpt_kvq8_cache* cache,
  * sequence (max_new * Hq / heads), each row's keys num_splits ways; with more,
  * the keys of all blocks of 128 rows in num_splits equal shares.  At most
  * 1024; <= 0: hipgpt_attn_kvq8_default_splits for max_len = max_pages *
- * page_size (T = batch in decode).  1 needs no workspace.
+ * page_size (T = batch in decode).  1 needs no workspace.  Calls that may run
+ * at the same time, replayed graphs among them, need workspaces of their own.
  * Sums and softmax statistics are fp32.  With an fp32 result the products are
  * off by 2^-22 of themselves at most; with a bf16 result the softmax weights
  * are rounded to fp16 first.  V scales are applied to those weights relative

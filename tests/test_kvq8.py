@@ -98,7 +98,7 @@ BAD_CACHES = [
 ]
 BAD_BATCHES = [
     (dict(block_table=0), 7), (dict(lens=0), 7), (dict(batch=0), 7), (dict(max_pages=0), 7), (dict(max_new=0), 7),
-    (dict(table_stride=-1), 7), (dict(table_stride=0), 7), (dict(), 0), (dict(), -3),
+    (dict(table_stride=-1), 7), (dict(table_stride=0), 7), (dict(table_stride=3), 7), (dict(), 0), (dict(), -3),
     (dict(cu_new=0, max_new=5), 2), (dict(cu_new=0, max_new=1), 3),
 ]
 
@@ -160,6 +160,9 @@ def test_attention_refusals():
     for kw in (dict(q=None), dict(o=None), dict(Hq=0), dict(Hq=3), dict(scale=float("nan")), dict(scale=float("inf")),
                dict(dt=2), dict(odt=-1)):
         assert both(**kw) == _lib.ERR_INVALID, kw
+    huge = batch(max_new=1 << 30)
+    assert L.hipgpt_attn_prefill_kvq8(cache(), huge, 1 << 30, P, P, 4, *s, *s, -1.0, 0, 0, 1, None, 0,
+                                      None) == _lib.ERR_UNSUPPORTED
     for kw in (dict(odt=1), dict(q=P + 4), dict(o=P + 8), dict(qs=(126, 64)), dict(os_=(128, 63)),
                dict(dt=1, odt=1, qs=(132, 64)), dict(c=cache(head_dim=48))):
         assert both(**kw) == _lib.ERR_UNSUPPORTED, kw

@@ -299,6 +299,13 @@ def test_advance(dev):
     b2 = K.Batch(c.d_table, b.lens, dev_t(np.array([0, 0, 1, 3], dtype=np.int32)), max_new=2)
     K.append(c.cache, b2, None, k, k, advance=True)
     assert host(b.lens).tolist() == [6, 2, 33]
+    # a slot without a sequence stays one, and nothing is stored for it
+    b3 = c.batch([6, -1, 2**31 - 1])
+    before = c.state()
+    K.append(c.cache, b3, None, k, k, advance=True)
+    assert host(b3.lens).tolist() == [7, -1, 2**31 - 1]
+    for w in "kv":
+        assert np.array_equal(c.state()[0][w][c.table[1:]], before[0][w][c.table[1:]])
 
 
 # ------------------------------------------------------------------- attention
@@ -427,7 +434,7 @@ def test_attention_bad_sequences(dev, call):
     q[5, 2, 0] = float("inf")
     new = [1] * 6
     b = c.batch(lens) if call == "decode" else c.batch(lens, new)
-    for kw in ([{}, {"num_splits": 3}] if call == "decode" else [{}]):
+    for kw in ({}, {"num_splits": 3}):
         got = host(getattr(K, call)(c.cache, b, q, **kw))
         check_attention(c, got, q64, lens, new, G, 0.125, "f32", skip=(1, 2, 3, 5))
         assert np.isnan(got[1:4]).all() and np.isnan(got[5, 1:3]).all()
@@ -638,3 +645,93 @@ def test_empty_slots(dev):
                   for w in "kv")
         want = R.attend(q64[1:2], kk.transpose(1, 0, 2)[:5], vv.transpose(1, 0, 2)[:5], 2, 0.125, 4)
         assert np.abs(got[1:2] - want).max() <= R.f32_tol(vv)
+
+
+@pytest.mark.parametrize("splits", [1, 7])
+def test_captured_prefill_replays(dev, splits):
+    """The 128-row blocks (whole and in shares) captured with an append: replays equal the eager
+    calls, with eager work of the program in between."""
+    H, ps, D, n = 2, 64, 128, 150
+    c = Case(111, [300, 20], [600, 200], H, ps, D)
+    lens, new = [300 + n, 20 + 60], [n, 60]
+    b = c.batch(lens, new)
+    q, k, v = (normal(c.rng, "bf16", sum(new), h, D)[0] for h in (4, H, H))
+    qr, out = torch.empty_like(q), torch.empty(sum(new), 4, D, device="cuda")
+    ws = torch.empty(max(1, K.workspace_bytes(sum(new), n, 4, H, D, splits)), dtype=torch.uint8, device="cuda")
+    f = K.rope_freqs(D)
+
+    def step():
+        K.append(c.cache, b, q, k, v, freqs=f, q_out=qr)
+        K.prefill(c.cache, b, qr, out=out, num_splits=splits, workspace=ws)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    torch.cuda.synchronize()
+    for i in range(4):
+        step()  # appending the same rows again leaves the codes as they are
+        want = out.clone()
+        out.fill_(float("nan"))
+        ws.fill_(255)  # what a workspace holds before a call does not matter
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+    check_attention(c, host(out), host(qr).astype(np.float64), lens, new, 2, D**-0.5, "f32", c.state())
+
+
+def test_streams_at_once(dev):
+    """Decode and prefill of two batches over one cache on two streams, workspaces of their own."""
+    lens = [1500, 900]
+    c = Case(121, lens, lens, 2, 64, 64)
+    q1, q64 = normal(c.rng, "f32", 2, 8, 64)
+    q2, p64 = normal(c.rng, "f32", 130, 8, 64)
+    new = [100, 30]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    b1, b2 = c.batch(lens), c.batch(lens, new)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        got.append((K.decode(c.cache, b1, q1, num_splits=6, stream=s1),
+                    K.prefill(c.cache, b2, q2, num_splits=9, stream=s2)))
+    torch.cuda.synchronize()
+    for a, b in got:
+        assert torch.equal(a, got[0][0]) and torch.equal(b, got[0][1])
+    check_attention(c, host(got[0][0]), q64, lens, [1, 1], 4, 0.125, "f32")
+    check_attention(c, host(got[0][1]), p64, lens, new, 4, 0.125, "f32")
+
+
+@pytest.mark.parametrize("dtype,out", TYPES)
+def test_mixed_batch_and_wide_tables(dev, dtype, out):
+    """Prompts beside single tokens and idle sequences; a table wider than its rows use."""
+    cached, new = [0, 500, 40, 7, 0], [200, 1, 0, 1, 33]
+    lens = [a + b for a, b in zip(cached, new)]
+    c = Case(131, lens, lens, 2, 32, 64)
+    wide = torch.full((5, c.table.shape[1] + 3), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c.table.shape[1]] = c.d_table
+    q, q64 = normal(c.rng, dtype, sum(new), 4, 64)
+    for splits in (1, 5):
+        b = c.batch(lens, new, table=wide[:, :c.table.shape[1]])
+        got = host(K.prefill(c.cache, b, q, out_dtype=DT[out], num_splits=splits))
+        check_attention(c, got, q64, lens, new, 2, 0.125, out)
+
+
+@pytest.mark.parametrize("call", ["decode", "prefill"])
+def test_zero_and_tiny_values(dev, call):
+    """Pages of zeros (scale 2^-126) among others: they count in the sums and add nothing."""
+    n, H, ps, D = 130, 1, 32, 64
+    c = Case(141, [n], [n], H, ps, D)
+    for j in (0, 2):
+        for w in "kv":
+            c.scale[w][c.table[0, j]] = np.float32(R.MIN_SCALE)
+    c.cache.k_scale.copy_(torch.from_numpy(c.scale["k"]))
+    c.cache.v_scale.copy_(torch.from_numpy(c.scale["v"]))
+    q, q64 = normal(c.rng, "f32", 1, 2, D)
+    wide = q.expand(1, 2, D).repeat(1, 20, 1)  # 40 rows of one head: the 128-row blocks in prefill
+    b = c.batch([n]) if call == "decode" else c.batch([n], [1])
+    got = host(getattr(K, call)(c.cache, b, wide))
+    k, v = c.rows("k", 0, n), c.rows("v", 0, n)
+    want = np.tile(R.attend(q64, k, v, 2, 0.125, n - 1), (1, 20, 1))
+    assert np.abs(got - want).max() <= R.f32_tol(v)
