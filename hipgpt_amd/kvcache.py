@@ -31,6 +31,7 @@ from .attention import _need_cuda, _ptr
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 # the stream handle alone: torch.cuda.current_stream() builds an object around it, 2.7 us a call
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _dtype(name, t):
@@ -131,19 +132,11 @@ def _rows(name, t, shape, dtype, device):
     return st[:2]
 
 
-def _on_device(call):
-    """Runs an entry point of this module with its cache's device current."""
-
-    @functools.wraps(call)
-    def run(cache, batch, *args, **kw):
-        if batch.device != cache.device:
-            raise ValueError("cache and batch must be on one device")
-        if torch.cuda.current_device() != cache.index:
-            with torch.cuda.device(cache.device):
-                return call(cache, batch, *args, **kw)
-        return call(cache, batch, *args, **kw)
-
-    return run
+def _enter(cache, batch):
+    """None where the cache's device is current, else a context that makes it so."""
+    if batch.device != cache.device:
+        raise ValueError("cache and batch must be on one device")
+    return None if _current_device() == cache.index else torch.cuda.device(cache.device)
 
 
 def _handle(cache, stream, *owned):
@@ -157,13 +150,16 @@ def _handle(cache, stream, *owned):
     return stream.cuda_stream
 
 
-@_on_device
 def append(cache, batch, q, k, v, freqs=None, interleaved=False, q_out=None, advance=False, stream=None):
     """Rotates and quantises the new tokens into the cache; returns the rotated q.
 
     k, v: [T, heads, D], q: [T, Hq, D] or None, all float32 or all bfloat16; ``freqs``:
     :func:`rope_freqs` of the rotated head dims (None: no rotation); ``q_out`` may be q.
     ``advance`` first raises ``batch.lens`` by the new tokens."""
+    other = _enter(cache, batch)
+    if other is not None:
+        with other:
+            return append(cache, batch, q, k, v, freqs, interleaved, q_out, advance, stream)
     _tensor("k", k)
     dt, dtype, dev = _dtype("k", k), k.dtype, cache.device
     T, D = k.shape[0], cache.head_dim
@@ -176,7 +172,7 @@ def append(cache, batch, q, k, v, freqs=None, interleaved=False, q_out=None, adv
         shape = (T, Hq, D)
         qs = _rows("q", q, shape, dtype, dev)
         if q_out is None:
-            q_out = mine = q.new_empty(shape)
+            q_out = mine = torch.empty_like(q)
         os_ = _rows("q_out", q_out, shape, dtype, dev)
         qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -194,10 +190,13 @@ def append(cache, batch, q, k, v, freqs=None, interleaved=False, q_out=None, adv
     return q_out
 
 
-@_on_device
 def read(cache, batch, T, dtype=torch.float32, k=None, v=None, stream=None):
     """(k, v) [T, heads, D]: the values of each sequence's last ``cu_new[b + 1] -
     cu_new[b]`` tokens, packed in that order (T rows in all)."""
+    other = _enter(cache, batch)
+    if other is not None:
+        with other:
+            return read(cache, batch, T, dtype, k, v, stream)
     shape = (T, cache.heads, cache.head_dim)
     mine = [None, None]
     if k is None:
@@ -225,6 +224,10 @@ def workspace_bytes(T, max_new, Hq, heads, D, num_splits):
 
 def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, workspace, stream):
     """Both attention entry points; ``rows``: (T,) where the entry point takes it."""
+    other = _enter(cache, batch)
+    if other is not None:
+        with other:
+            return _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, workspace, stream)
     T, Hq, _ = q.shape
     H, D, dev = cache.heads, cache.head_dim, cache.device
     shape = (T, Hq, D)
@@ -232,7 +235,7 @@ def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, w
     qs = _rows("q", q, shape, q.dtype, dev)
     mine = [None, None]
     if out is None:
-        out = mine[0] = q.new_empty(shape, dtype=out_dtype)
+        out = mine[0] = torch.empty(shape, dtype=out_dtype, device=dev)
     os_ = _rows("out", out, shape, out.dtype, dev)
     if num_splits is None:
         num_splits = default_splits(batch.size, T, batch.max_new, Hq, H, D, batch.max_len or batch.capacity(cache))
@@ -251,7 +254,6 @@ def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, w
     return out
 
 
-@_on_device
 def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
            stream=None):
     """softmax(q k^T * scale) v of q [B, Hq, D] over each sequence's cached tokens.
@@ -266,7 +268,6 @@ def decode(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_s
                       stream)
 
 
-@_on_device
 def prefill(cache, batch, q, out=None, out_dtype=torch.float32, scale=None, num_splits=None, workspace=None,
             stream=None):
     """Causal attention of each sequence's new tokens (q [T, Hq, D], packed as
