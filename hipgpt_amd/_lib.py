@@ -88,8 +88,8 @@ SIGNATURES = {
     "hipgpt_kvq8_append": (
         _int, [_vp, _vp, _int] + [_vp] * 4 + [_int] + [_i64] * 8 + [_vp, _int, _int, _int, _int, _vp]),
     "hipgpt_kvq8_read": (_int, [_vp, _vp, _int, _vp, _vp] + [_i64] * 4 + [_int, _vp]),
-    "hipgpt_attn_kvq8_default_splits": (_int, [_int] * 7),
-    "hipgpt_attn_kvq8_workspace_bytes": (_sz, [_int] * 6),
+    "hipgpt_attn_kvq8_default_splits": (_int, [_int] * 8),
+    "hipgpt_attn_kvq8_workspace_bytes": (_sz, [_int] * 8),
     "hipgpt_attn_decode_kvq8": (
         _int, [_vp, _vp, _vp, _vp, _int] + [_i64] * 4 + [_f, _int, _int, _int, _vp, _sz, _vp]),
     "hipgpt_attn_prefill_kvq8": (

@@ -118,9 +118,9 @@ hipError_t launch_advance(int* lens, const int* cu, int B, hipStream_t s);
 // kvq8_attn.hip) split the keys of each 16-row tile nsplit ways; more rows
 // (launch_tiles) take 128-row blocks, whole with nsplit 1, else as nsplit equal
 // shares of all their keys.
-bool tiles_for(int max_new, int G);
-int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int max_len);
-size_t attn_workspace(int T, int max_new, int Hq, int Hkv, int D, int nsplit);
+bool tiles_for(int B, int max_new, int Hq, int Hkv, int out_dtype);
+int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int out_dtype, int max_len);
+size_t attn_workspace(int B, int T, int max_new, int Hq, int Hkv, int D, int out_dtype, int nsplit);
 hipError_t launch_attn(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s);
 hipError_t launch_tiles(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s);
 int tile_shares(int D);

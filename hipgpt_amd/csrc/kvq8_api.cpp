@@ -71,9 +71,10 @@ int attention(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, con
     if (!rows16(q, q_ts, q_hs, dtype) || !rows16(o, o_ts, o_hs, out_dtype)) return HIPGPT_ERR_UNSUPPORTED;
     const int64_t cap = (int64_t)k.max_pages << k.lps;
     int ns = num_splits > 0 ? num_splits
-                            : kvq8::attn_splits(k.B, k.T, k.max_new, Hq, k.H, k.D, cap > 0x7fffffff ? 0x7fffffff : (int)cap);
+                            : kvq8::attn_splits(k.B, k.T, k.max_new, Hq, k.H, k.D, out_dtype,
+                                                cap > 0x7fffffff ? 0x7fffffff : (int)cap);
     if (ns > kvq8::kMaxSplits) ns = kvq8::kMaxSplits;
-    const size_t need = kvq8::attn_workspace(k.T, k.max_new, Hq, k.H, k.D, ns);
+    const size_t need = kvq8::attn_workspace(k.B, k.T, k.max_new, Hq, k.H, k.D, out_dtype, ns);
     if (need > 0 && (!ws || ws_bytes < need)) return HIPGPT_ERR_WORKSPACE;
     if (need > 0 && !aligned(ws, 16)) return HIPGPT_ERR_UNSUPPORTED;
     kvq8::AttnArgsQ8 a{};
@@ -156,15 +157,16 @@ int hipgpt_kvq8_read(const hipgpt_kvq8_cache* cache, const hipgpt_kvq8_batch* ba
     return from_hip(kvq8::launch_read(c, a, dtype, stream));
 }
 
-int hipgpt_attn_kvq8_default_splits(int B, int T, int max_new, int Hq, int heads, int D, int max_len) {
+int hipgpt_attn_kvq8_default_splits(int B, int T, int max_new, int Hq, int heads, int D, int out_dtype, int max_len) {
     if (B <= 0 || T <= 0 || max_new <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0 || max_len <= 0)
         return 1;
-    return kvq8::attn_splits(B, T, max_new < T ? max_new : T, Hq, heads, D, max_len);
+    return kvq8::attn_splits(B, T, max_new < T ? max_new : T, Hq, heads, D, out_dtype, max_len);
 }
 
-size_t hipgpt_attn_kvq8_workspace_bytes(int T, int max_new, int Hq, int heads, int D, int num_splits) {
-    if (T <= 0 || max_new <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0) return 0;
-    return kvq8::attn_workspace(T, max_new < T ? max_new : T, Hq, heads, D,
+size_t hipgpt_attn_kvq8_workspace_bytes(int B, int T, int max_new, int Hq, int heads, int D, int out_dtype,
+                                        int num_splits) {
+    if (B <= 0 || T <= 0 || max_new <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0) return 0;
+    return kvq8::attn_workspace(B, T, max_new < T ? max_new : T, Hq, heads, D, out_dtype,
                                 num_splits < kvq8::kMaxSplits ? num_splits : kvq8::kMaxSplits);
 }
 

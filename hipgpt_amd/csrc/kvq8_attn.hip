@@ -18,6 +18,14 @@
 // own in the same product (8 rows a tile instead of 16), and the two halves
 // are added once per score and once at the end.
 //
+// Bound by memory: a copy of the kernel that only loads the codes takes as long.
+// 64 sequences of 512 .. 8192 keys, 32/8 heads D128 bf16 (572 MB) 107 us + 5 us
+// join, 5.3 TB/s; 2 of 65537 and 131072 keys 78 + 6 us; 64 of up to 2048, 12 heads
+// D64 fp32 (101 MB) 26 us, where the longest sequence decides (loads alone 22);
+// one of 333 keys 6.1 us, three loads' latency and the launch.  Equal shares of
+// all keys in place of splits (as kvq8_tiles.hip has them) lost: 118 + 7, 85 + 5
+// and 37 us.
+//
 // S^T = K Q^T (16 tokens x 16 rows): lane (c, q) of the accumulator holds
 // tokens 4q..4q+3 of row c; two such products make the 32-token B operand of
 // O^T = V^T P^T without leaving registers, the cache's V tiles being in that
@@ -33,7 +41,7 @@ namespace kvq8 {
 
 namespace {
 
-constexpr int NW = 4;  // waves per workgroup
+constexpr int NW = 4;  // waves per workgroup (8: 572 MB above 108 -> 115 us, one of 1000 keys 10.3 -> 9.1)
 
 __device__ __forceinline__ float xor8_add(float x) {  // + the lane 8 places away in its row of 16
     const int y = __builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false);
@@ -385,7 +393,7 @@ hipError_t launch_rows(const Cache& c, const AttnArgsQ8& a, hipStream_t s) {
 template <int D>
 hipError_t launch_dim(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s) {
         hipError_t e;
-    if (tiles_for(c.max_new, a.Hq / c.H)) return launch_tiles(c, a, dtype, out_dtype, s);
+    if (tiles_for(c.B, c.max_new, a.Hq, c.H, out_dtype)) return launch_tiles(c, a, dtype, out_dtype, s);
     if (dtype == kF32)
         e = launch_rows<D, 2, float, float>(c, a, s);
     else if (out_dtype == kF32)
@@ -398,16 +406,34 @@ hipError_t launch_dim(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dt
 
 }  // namespace
 
-// Whether so many rows of one cached head take the 128-row blocks.
-bool tiles_for(int max_new, int G) { return (int64_t)max_new * G > 32; }
+// 16-row tiles (8 with an fp32 result) that the rows of one cached head fill.
+static int64_t row_tiles(int max_new, int G, int out_dtype) {
+    const int rpb = out_dtype == kF32 ? 8 : 16;
+    return ((int64_t)max_new * G + rpb - 1) / rpb;
+}
 
-int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int max_len) {
-    const int64_t G = Hq / Hkv;
-    if (tiles_for(max_new, (int)G)) {
-        const int64_t blocks = Hkv * (T * G / 128 + B);  // row blocks, at most
-        return blocks < tile_shares(D) && max_len >= 1024 ? tile_shares(D) : 1;
+// Whether the rows take the 128-row blocks.  One 16-row tile reads the codes
+// once and needs no LDS; several read them again each, which pays only while
+// they leave most CUs idle.  us, 16-row tiles / 128-row blocks, 8 heads D128
+// bf16, 8 | 16 | 32 | 48 rows: 64 sequences of 2048-4096 keys 73 / 120 | 77 / 119 |
+// 153 / 119 | 219 / 135, 4 of 4096-8192 21 / 40 | 22 / 41 | 32 / 42 | 45 / 46; fp32,
+// 8 | 16 | 24 | 32 rows: 77 / 142 | 153 / 142 | 221 / 143 | 289 / 142 and 21 / 46 |
+// 33 / 47 | 45 / 48 | 53 / 49.
+bool tiles_for(int B, int max_new, int Hq, int Hkv, int out_dtype) {
+    const int64_t n = row_tiles(max_new, Hq / Hkv, out_dtype);
+    return n > 3 || (n > 1 && (int64_t)B * Hkv * n > 256);
+}
+
+int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int out_dtype, int max_len) {
+    if (max_len <= 1024) return 1;
+    if (tiles_for(B, max_new, Hq, Hkv, out_dtype)) {
+        // shares where whole blocks are fewer than the device holds at once (1289
+        // rows of 32/8 heads behind 4-8k keys: 311 us whole in two splits, 236 in
+        // shares; 1024 blocks of 2048 keys: 108 us whole, 152 in shares)
+        const int64_t blocks = Hkv * (T * (int64_t)(Hq / Hkv) / 128 + B);  // at most
+        return blocks < tile_shares(D) ? tile_shares(D) : 1;
     }
-    const int64_t wgs = Hkv * B * ((max_new * G + 15) / 16);
+    const int64_t wgs = Hkv * B * row_tiles(max_new, Hq / Hkv, out_dtype);
     // One workgroup per CU at least, none with fewer than 256 keys (the join is
     // a launch of ~3 us: 1000 keys of 12 heads D64 10.5 us whole, 10.8 in two),
     // and two per CU where whole rows are so long that the longest of them
@@ -415,15 +441,15 @@ int attn_splits(int B, int T, int max_new, int Hq, int Hkv, int D, int max_len) 
     // More splits lose: 2 sequences of 131072 and 65537 keys 83 / 83 / 87 / 96 us
     // at 16 / 32 / 64 / 128.
     int n = 1;
-    while (n < 256 && max_len / (2 * n) >= 256 && max_len > 1024 &&
+    while (n < 256 && max_len / (2 * n) >= 256 &&
            (wgs * n < 256 || (wgs * n <= 512 && max_len / n >= 8192)))
         n *= 2;
     return n;
 }
 
-size_t attn_workspace(int T, int max_new, int Hq, int Hkv, int D, int nsplit) {
+size_t attn_workspace(int B, int T, int max_new, int Hq, int Hkv, int D, int out_dtype, int nsplit) {
     if (nsplit <= 1) return 0;
-    if (tiles_for(max_new, Hq / Hkv)) return tile_workspace(D, nsplit);
+    if (tiles_for(B, max_new, Hq, Hkv, out_dtype)) return tile_workspace(D, nsplit);
     return (size_t)T * Hq * nsplit * (size_t)(D + 2) * sizeof(float);
 }
 

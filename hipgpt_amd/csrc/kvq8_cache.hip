@@ -15,8 +15,15 @@
 //   append_pages_kernel: one workgroup per page, K or V, and group of heads;
 //     32 values a thread.  A thread keeps its place in the page from head to
 //     head, so it forms its sines and cosines once for all the heads (K's and
-//     the queries') of its group.
-//   append_token_kernel: one token per sequence; a wave per row.
+//     the queries') of its group.  Bound by memory and the maximum's barriers:
+//     11793 tokens of 16 + 16 heads D128 bf16 (241 MB in and out) 84 us, 2.9 TB/s
+//     where a large copy reaches 4.8; 1 / 2 / 4 heads a group 110 / 90 / 84, the
+//     next head's rows requested early 88 (31 more registers).
+//   append_token_kernel: one token per sequence; a wave per row.  Bound by the
+//     latency of length -> page -> scale: 64 sequences, 32 + 8 heads D128 4.8 us,
+//     one sequence 3.6.
+// read_kernel: bound by memory, 56772 tokens of 8 heads D128 to bf16 (349 MB)
+// 78 us, 4.5 TB/s.
 #include "common.h"
 #include "kernels.h"
 #include "kvq8.h"

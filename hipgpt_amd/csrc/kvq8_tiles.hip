@@ -3,6 +3,16 @@
 // operands are those of kvq8_attn.hip; here the products are 32x32x16 and the
 // codes become fp16 once per workgroup, in LDS.
 //
+// What bounds it: matrix and vector work of a SIMD's waves hardly overlap on
+// this chip, so a wave costs their sum.  At D = 128, bf16 in and out, 64 tokens x
+// 32 rows are 32 MFMAs (1024 cycles) and ~280 vector instructions, 32 of them
+// exponentials (~1450): 512 equal workgroups, two a CU, take 2.7 us per stage
+// pair (790 TFLOP/s) where that sum is 2.1.  fp32 in and out doubles the MFMAs.
+// Measured: 4 prompts of 2048 tokens, 16 heads D128 bf16 105 us (655 TFLOP/s);
+// 8 of 1024, 12 heads D64 fp32 43 us.  128 rows a workgroup: the codes' way to
+// fp16 costs 72 of the 280, shared by its four waves; eight waves (256 rows)
+// measured level at D = 128 and 10% slower at D = 64, whose codes are half.
+//
 // A workgroup holds 4 waves x 32 rows (token i, query head g, in the order
 // i * G + g, so that the heads that share a cached head share its tiles) and
 // walks the keys 64 at a time: codes of the next 64 are in flight to registers

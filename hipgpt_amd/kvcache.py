@@ -213,13 +213,14 @@ def read(cache, batch, T, dtype=torch.float32, k=None, v=None, stream=None):
 
 
 @functools.lru_cache(maxsize=4096)
-def default_splits(B, T, max_new, Hq, heads, D, max_len):
+def default_splits(B, T, max_new, Hq, heads, D, out_dtype, max_len):
     """The split count that the library picks for these sizes."""
-    return int(_lib.lib().hipgpt_attn_kvq8_default_splits(B, T, max_new, Hq, heads, D, max_len))
+    return int(_lib.lib().hipgpt_attn_kvq8_default_splits(B, T, max_new, Hq, heads, D, _TYPES[out_dtype], max_len))
 
 
-def workspace_bytes(T, max_new, Hq, heads, D, num_splits):
-    return int(_lib.lib().hipgpt_attn_kvq8_workspace_bytes(T, max_new, Hq, heads, D, num_splits))
+def workspace_bytes(B, T, max_new, Hq, heads, D, out_dtype, num_splits):
+    return int(_lib.lib().hipgpt_attn_kvq8_workspace_bytes(B, T, max_new, Hq, heads, D, _TYPES[out_dtype],
+                                                           num_splits))
 
 
 def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, workspace, stream):
@@ -237,17 +238,20 @@ def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, w
     if out is None:
         out = mine[0] = torch.empty(shape, dtype=out_dtype, device=dev)
     os_ = _rows("out", out, shape, out.dtype, dev)
+    odt = _dtype("out", out)
     if num_splits is None:
-        num_splits = default_splits(batch.size, T, batch.max_new, Hq, H, D, batch.max_len or batch.capacity(cache))
+        num_splits = default_splits(batch.size, T, batch.max_new, Hq, H, D, out.dtype,
+                                    batch.max_len or batch.capacity(cache))
     ns = int(num_splits)
     wp = nbytes = 0
     if ns > 1:
         if workspace is None:
-            workspace = mine[1] = q.new_empty(workspace_bytes(T, batch.max_new, Hq, H, D, ns), dtype=torch.uint8)
+            need = workspace_bytes(batch.size, T, batch.max_new, Hq, H, D, out.dtype, ns)
+            workspace = mine[1] = torch.empty(need, dtype=torch.uint8, device=dev)
         wp, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     rc = getattr(_lib.lib(), name)(
         cache._ref, batch._ref, *rows, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_,
-        -1.0 if scale is None else float(scale), dt, _dtype("out", out), 1 if ns < 1 else ns, wp, nbytes,
+        -1.0 if scale is None else float(scale), dt, odt, 1 if ns < 1 else ns, wp, nbytes,
         _handle(cache, stream, *mine))
     if rc:
         _lib.check(rc, name)

@@ -278,21 +278,23 @@ int hipgpt_kvq8_read(const hipgpt_kvq8_cache* cache,
  *   fp32 o.  scale <= 0 selects 1/sqrt(D).
  * num_splits > 1 divides the work and joins the parts by a second kernel
  * through a caller-owned, 16-byte aligned workspace of
- * hipgpt_attn_kvq8_workspace_bytes: up to 32 query rows per cached head and
- * sequence (max_new * Hq / heads), each row's keys num_splits ways; with more,
- * the keys of all blocks of 128 rows in num_splits equal shares.  At most
- * 1024; <= 0: hipgpt_attn_kvq8_default_splits for max_len = max_pages *
- * page_size (T = batch in decode).  1 needs no workspace.  Calls that may run
- * at the same time, replayed graphs among them, need workspaces of their own.
+ * hipgpt_attn_kvq8_workspace_bytes: with few query rows per cached head and
+ * sequence, each row's keys num_splits ways; with more, the keys of all blocks
+ * of 128 rows in num_splits equal shares.  At most 1024; <= 0:
+ * hipgpt_attn_kvq8_default_splits for max_len = max_pages * page_size (in
+ * decode T = B and max_new = 1).  1 needs no workspace.  Calls that may run at
+ * the same time, replayed graphs among them, need workspaces of their own.
  * Sums and softmax statistics are fp32.  With an fp32 result the products are
  * off by 2^-22 of themselves at most; with a bf16 result the softmax weights
  * are rounded to fp16 first.  V scales are applied to those weights relative
  * to the largest scale that the row's block of rows met, so what pages with
  * scales under 2^-24 of it contribute is lost in part (fp16's range). */
 int hipgpt_attn_kvq8_default_splits(int B, int T, int max_new, int Hq,
-                                    int heads, int D, int max_len);
-size_t hipgpt_attn_kvq8_workspace_bytes(int T, int max_new, int Hq, int heads,
-                                        int D, int num_splits);
+                                    int heads, int D, int out_dtype,
+                                    int max_len);
+size_t hipgpt_attn_kvq8_workspace_bytes(int B, int T, int max_new, int Hq,
+                                        int heads, int D, int out_dtype,
+                                        int num_splits);
 int hipgpt_attn_decode_kvq8(const hipgpt_kvq8_cache* cache,
                             const hipgpt_kvq8_batch* batch, const void* q,
                             void* o, int Hq, int64_t q_ts, int64_t q_hs,

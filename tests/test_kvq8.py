@@ -173,22 +173,31 @@ def test_attention_refusals():
     assert dec(cache(), None, P, P, 4, *s, *s, -1.0, 0, 0, 1, None, 0, None) == _lib.ERR_INVALID
     assert dec(None, batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 1, None, 0, None) == _lib.ERR_INVALID
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, None, 0, None) == _lib.ERR_WORKSPACE
-    wb = L.hipgpt_attn_kvq8_workspace_bytes
+    def wb(B, T, new, Hq, H, D, ns, odt=0):
+        return L.hipgpt_attn_kvq8_workspace_bytes(B, T, new, Hq, H, D, odt, ns)
+
     # parts of every row where few rows share a cached head, else two slots of 128 rows a share
-    need = wb(2, 1, 4, 2, 64, 3)
+    need = wb(2, 2, 1, 4, 2, 64, 3)
     assert need == 2 * 4 * 3 * 66 * 4
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, P, need - 4, None) == _lib.ERR_WORKSPACE
     assert dec(cache(), batch(**one), P, P, 4, *s, *s, -1.0, 0, 0, 3, P + 4, need, None) == _lib.ERR_UNSUPPORTED
-    assert wb(2, 1, 4, 2, 64, 1) == wb(0, 1, 4, 2, 64, 4) == wb(2, 1, 5, 2, 64, 4) == 0
-    assert wb(2, 1, 4, 2, 64, 5000) == wb(2, 1, 4, 2, 64, 1024)
+    assert wb(2, 2, 1, 4, 2, 64, 1) == wb(2, 0, 1, 4, 2, 64, 4) == wb(2, 2, 1, 5, 2, 64, 4) == 0
+    assert wb(2, 2, 1, 4, 2, 64, 5000) == wb(2, 2, 1, 4, 2, 64, 1024)
     pre = L.hipgpt_attn_prefill_kvq8
-    need = wb(70, 50, 4, 2, 64, 3)
+    need = wb(2, 70, 50, 4, 2, 64, 3)
     assert need == 3 * (4 + 2 * 128 * (64 + 4)) * 4
     assert pre(cache(), batch(max_new=50), 70, P, P, 4, *s, *s, -1.0, 0, 0, 3, P, need - 4, None) == _lib.ERR_WORKSPACE
-    ds = L.hipgpt_attn_kvq8_default_splits
+    # 16 rows of a cached head: one tile with a bf16 result, two with an fp32 one, which pay in small batches only
+    assert wb(64, 256, 4, 32, 8, 128, 3, 1) == 256 * 32 * 3 * 130 * 4
+    assert wb(4, 16, 4, 32, 8, 128, 3, 0) == 16 * 32 * 3 * 130 * 4
+    assert wb(64, 256, 4, 32, 8, 128, 3, 0) == 3 * (4 + 2 * 128 * 132) * 4
+
+    def ds(B, T, new, Hq, H, D, ln, odt=0):
+        return L.hipgpt_attn_kvq8_default_splits(B, T, new, Hq, H, D, odt, ln)
+
     assert ds(2, 2, 1, 5, 4, 64, 1 << 20) == 1  # heads that do not divide
     assert ds(0, 2, 1, 4, 4, 64, 99999) == ds(2, 0, 1, 4, 4, 64, 99999) == ds(2, 2, 0, 4, 4, 64, 99999) == 1
-    assert ds(1, 1, 1, 8, 8, 64, 100) == 1
+    assert ds(1, 1, 1, 8, 8, 64, 1024) == 1
     assert 16 <= ds(1, 1, 1, 8, 8, 64, 1 << 17) <= 256
     assert ds(1, 4096, 4096, 8, 8, 128, 1 << 15) == 512 and ds(64, 65536, 1024, 8, 8, 128, 1024) == 1
     assert ds(1, 500, 500, 8, 8, 128, 1000) == 1

@@ -553,7 +553,7 @@ def test_captured_steps_replay(dev):
     f = K.rope_freqs(D)
     q, k, v = (normal(c.rng, "f32", B, H, D)[0] for _ in range(3))
     out, out2, qr = (torch.empty(B, H, D, device="cuda") for _ in range(3))
-    ws = torch.empty(K.workspace_bytes(B, 1, H, H, D, 4), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(K.workspace_bytes(B, B, 1, H, H, D, torch.float32, 4), dtype=torch.uint8, device="cuda")
     lens = dev_t(np.array([40, 7, 0], dtype=np.int32))
     cu = dev_t(np.arange(B + 1, dtype=np.int32))
 
@@ -657,7 +657,7 @@ def test_captured_prefill_replays(dev, splits):
     b = c.batch(lens, new)
     q, k, v = (normal(c.rng, "bf16", sum(new), h, D)[0] for h in (4, H, H))
     qr, out = torch.empty_like(q), torch.empty(sum(new), 4, D, device="cuda")
-    ws = torch.empty(max(1, K.workspace_bytes(sum(new), n, 4, H, D, splits)), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(max(1, K.workspace_bytes(2, sum(new), n, 4, H, D, torch.float32, splits)), dtype=torch.uint8, device="cuda")
     f = K.rope_freqs(D)
 
     def step():
