@@ -19,6 +19,12 @@ bool rows16(const void* p, int64_t ts, int64_t hs, int dtype) {
     return aligned(p, 16) && ts % n == 0 && hs % n == 0;
 }
 
+// (n - 1) * stride, n > 0 and stride > 0, at most 2^62
+int64_t spread(int64_t n, int64_t stride) {
+    const int64_t most = (int64_t)1 << 62;
+    return n > 1 && stride > most / (n - 1) ? most : (n - 1) * stride;
+}
+
 // The cache and batch as the kernels take them; T: rows of the packed buffers.
 int problem(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, kvq8::Cache& out) {
     if (!c || !b || !c->k || !c->v || !c->k_scale || !c->v_scale || !b->block_table || !b->lens)
@@ -31,6 +37,13 @@ int problem(const hipgpt_kvq8_cache* c, const hipgpt_kvq8_batch* b, int T, kvq8:
     if (!kvq8::supported(c->head_dim, c->page_size)) return HIPGPT_ERR_UNSUPPORTED;
     const int64_t bytes = (int64_t)c->page_size * c->head_dim;
     if (c->head_stride < bytes || c->page_stride < bytes || c->scale_page_stride < 1 || c->scale_head_stride < 1)
+        return HIPGPT_ERR_INVALID;
+    // pages and heads apart: heads inside a page's stride, or pages inside a head's
+    if (c->page_stride < spread(c->heads, c->head_stride) + bytes &&
+        c->head_stride < spread(c->num_pages, c->page_stride) + bytes)
+        return HIPGPT_ERR_INVALID;
+    if (c->scale_page_stride < spread(c->heads, c->scale_head_stride) + 1 &&
+        c->scale_head_stride < spread(c->num_pages, c->scale_page_stride) + 1)
         return HIPGPT_ERR_INVALID;
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % 16 || c->head_stride % 16)
         return HIPGPT_ERR_UNSUPPORTED;

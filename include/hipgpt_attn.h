@@ -187,7 +187,9 @@ int hipgpt_attn_decode_kvcache(const float* q, const float* k_new,
  * head_dim D in {32, 64, 128, 256}.
  *   k, v:    element (page, head) at X + page * page_stride + head *
  *            head_stride, page_size * D bytes each; 16-byte aligned, strides
- *            multiples of 16.  K is [token][D]; V is [token / 32][D / 32][4]
+ *            multiples of 16.  All heads of a page lie within a page_stride,
+ *            or all pages of a head within a head_stride.
+ *            K is [token][D]; V is [token / 32][D / 32][4]
  *            [16][2][2][4], where token % 32 = 16 i3 + 4 i0 + i4 and d % 32 =
  *            16 i2 + i1 of the last five indexes i0 .. i4.
  *   scales:  (page, head) at S[page * scale_page_stride + head *

@@ -94,7 +94,12 @@ BAD_CACHES = [
     (dict(page_size=256), "UNSUPPORTED"), (dict(head_dim=48), "UNSUPPORTED"), (dict(head_dim=512), "UNSUPPORTED"),
     (dict(head_stride=64 * 64 - 16), "INVALID"), (dict(page_stride=0), "INVALID"), (dict(scale_page_stride=0), "INVALID"),
     (dict(scale_head_stride=0), "INVALID"), (dict(k=P + 8), "UNSUPPORTED"), (dict(v=P + 4), "UNSUPPORTED"),
-    (dict(head_stride=64 * 64 + 8), "UNSUPPORTED"), (dict(page_stride=2 * 64 * 64 + 4), "UNSUPPORTED"),
+    (dict(page_stride=3 * 64 * 64, head_stride=64 * 64 + 8), "UNSUPPORTED"),
+    (dict(page_stride=2 * 64 * 64 + 4), "UNSUPPORTED"),
+    # heads and pages that overlap
+    (dict(page_stride=64 * 64), "INVALID"), (dict(page_stride=2 * 64 * 64, head_stride=64 * 64 + 16), "INVALID"),
+    (dict(page_stride=64 * 64, head_stride=3 * 64 * 64), "INVALID"), (dict(scale_page_stride=1), "INVALID"),
+    (dict(page_stride=1 << 62, head_stride=1 << 62), "INVALID"),
 ]
 BAD_BATCHES = [
     (dict(block_table=0), 7), (dict(lens=0), 7), (dict(batch=0), 7), (dict(max_pages=0), 7), (dict(max_new=0), 7),

@@ -735,3 +735,21 @@ def test_zero_and_tiny_values(dev, call):
     k, v = c.rows("k", 0, n), c.rows("v", 0, n)
     want = np.tile(R.attend(q64, k, v, 2, 0.125, n - 1), (1, 20, 1))
     assert np.abs(got - want).max() <= R.f32_tol(v)
+
+
+def test_pools_by_head(dev):
+    """Pools laid out [heads][pages] and scales likewise, seen as [pages, heads]."""
+    lens, new = [70, 33], [70, 3]
+    c = Case(151, [0, 30], lens, 3, 32, 64)
+    t = c.cache
+    codes = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (t.k, t.v)]
+    scales = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (t.k_scale, t.v_scale)]
+    c.cache = K.CacheQ8(*codes, *scales)
+    q, q64 = normal(c.rng, "bf16", 73, 6, 64)
+    k, k64 = normal(c.rng, "bf16", 73, 3, 64)
+    v, v64 = normal(c.rng, "bf16", 73, 3, 64)
+    before = c.state()
+    K.append(c.cache, c.batch(lens, new), None, k, v)
+    check_append(c, lens, new, {"k": k64, "v": v64}, 0, False, before, c.state())
+    got = host(K.prefill(c.cache, c.batch(lens, new), q))
+    check_attention(c, got, q64, lens, new, 2, 0.125, "f32", c.state())
