@@ -11,19 +11,24 @@
 // point, so p * f_i mod 2^64 is the exact fraction of a turn at any position.
 //
 // Both kernels read each row once and keep its values in registers between the
-// maximum and the rounding.
+// maximum and the rounding.  Rows are read non-temporally: what stays near is
+// the codes, which are read next (11793 tokens of 16 heads D128 read back: 33 -> 25
+// us), and the append itself is 6% faster.
 //   append_pages_kernel: one workgroup per page, K or V, and group of heads;
 //     32 values a thread.  A thread keeps its place in the page from head to
 //     head, so it forms its sines and cosines once for all the heads (K's and
 //     the queries') of its group.  Bound by memory and the maximum's barriers:
-//     11793 tokens of 16 + 16 heads D128 bf16 (241 MB in and out) 84 us, 2.9 TB/s
-//     where a large copy reaches 4.8; 1 / 2 / 4 heads a group 110 / 90 / 84, the
-//     next head's rows requested early 88 (31 more registers).
+//     11793 tokens of 16 + 16 heads D128 bf16 (241 MB in and out) 67 us, 3.6 TB/s
+//     where a large copy reaches 4.8; 2 / 4 / 8 heads a group 67 / 67 / 68 (1: 40%
+//     more), the queries in workgroups of their own 73, the next head's rows
+//     requested early level, groups of 16 neighbouring head dims (lanes 32 bytes
+//     apart) 7% slower.
 //   append_token_kernel: one token per sequence; a wave per row.  Bound by the
 //     latency of length -> page -> scale: 64 sequences, 32 + 8 heads D128 4.8 us,
 //     one sequence 3.6.
 // read_kernel: bound by memory, 56772 tokens of 8 heads D128 to bf16 (349 MB)
-// 78 us, 4.5 TB/s.
+// 78 us, 4.5 TB/s; non-temporal stores 60, but what reads the rows next takes that
+// much longer (and 39 -> 44 us for both at 64 MB, fp32 rows 20 -> 46 alone).
 #include "common.h"
 #include "kernels.h"
 #include "kvq8.h"
@@ -67,7 +72,7 @@ struct Vec<__bf16> {
 
 template <class T>
 __device__ __forceinline__ void load4(const T* p, float* x) {
-    const typename Vec<T>::v4 v = *reinterpret_cast<const typename Vec<T>::v4*>(p);
+    const typename Vec<T>::v4 v = __builtin_nontemporal_load(reinterpret_cast<const typename Vec<T>::v4*>(p));
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
 }
@@ -140,27 +145,33 @@ __device__ void recode_page(uint8_t* codes, bool is_v, int n, int D, float r, in
     }
 }
 
-// 16 values of a row: head dims dim(j), j = 0 .. 15, of which j and j + 8 (or,
-// interleaved, 2i and 2i + 1) are a rotated pair.  Where the pairs lie rot / 2
-// apart and that is no multiple of 8 (ODD), groups hold what is left over and
-// head dims are taken one by one.
-template <bool ODD>
+// Where a row's rotated pairs are: (2i, 2i + 1) (or none), (i, i + rot / 2) with
+// rot / 2 a multiple of 8, or any other rot / 2.
+enum { kPairs, kHalves, kOdd };
+
+// 16 values of a row: head dims d0 .. d0 + 7 and d1 .. d1 + 7, so that a wave's
+// loads have no gaps; values j and j + 8 (kPairs: 2i and 2i + 1) are a rotated
+// pair.  With kOdd, groups hold what is left over and head dims are taken one
+// by one.
+template <int MODE>
 struct Group {
-    int d0, d1;   // first head dim of j < 8 and of j >= 8
-    int n0, n1;   // valid ones of each (ODD)
-    int pair;     // first pair, or -1
+    static constexpr bool ODD = MODE == kOdd;
+    int d0, d1;  // first head dim of j < 8 and of j >= 8
+    int n0, n1;  // valid ones of each (ODD)
+    int pair, pair4;  // first and fifth of the eight pairs, or -1
     __device__ __forceinline__ void init(int g, int D, const AppendArgs& a) {
         n0 = n1 = 8;
-        pair = -1;
+        pair = pair4 = -1;
         const int half = a.rot >> 1;
-        if (a.rot == 0 || a.interleaved) {
-            d0 = 16 * g;
-            d1 = d0 + 8;
-            if (a.rot) pair = 8 * g;
+        if (MODE == kPairs) {
+            d0 = 8 * g;
+            d1 = d0 + D / 2;
+            if (a.rot) pair = d0 / 2, pair4 = d1 / 2;
         } else {
             const int ng = (half + 7) >> 3;
             if (g < ng) {
                 pair = d0 = 8 * g;
+                pair4 = pair + 4;
                 d1 = d0 + half;
                 if (ODD) n0 = n1 = min(8, half - d0);
             } else {
@@ -220,36 +231,39 @@ struct Group {
         for (int j = 0; j < 8; ++j) {
             c[j] = 1.f;
             s[j] = 0.f;
-            if (pair >= 0 && pair + j < (a.rot >> 1)) turn(a.freqs[pair + j], pos, c[j], s[j]);
+            const int p = j < 4 ? pair + j : pair4 + j - 4;
+            if (pair >= 0 && p < (a.rot >> 1)) turn(a.freqs[p], pos, c[j], s[j]);
         }
     }
     __device__ __forceinline__ void rotate(const AppendArgs& a, float* x, const float* c, const float* s) const {
         if (pair < 0) return;
-        const int n = (a.rot >> 1) - pair;
+        const int half = a.rot >> 1;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             // pair j: (j, j + 8) or (2j, 2j + 1)
-            float& p = a.interleaved ? x[2 * j] : x[j];
-            float& q = a.interleaved ? x[2 * j + 1] : x[j + 8];
+            float& p = MODE == kPairs ? x[2 * j] : x[j];
+            float& q = MODE == kPairs ? x[2 * j + 1] : x[j + 8];
             const float p0 = p, q0 = q;
-            p = j < n ? fmaf(p0, c[j], -(q0 * s[j])) : p0;
-            q = j < n ? fmaf(q0, c[j], p0 * s[j]) : q0;
+            const bool on = (j < 4 ? pair + j : pair4 + j - 4) < half;
+            p = on ? fmaf(p0, c[j], -(q0 * s[j])) : p0;
+            q = on ? fmaf(q0, c[j], p0 * s[j]) : q0;
         }
     }
 };
 
-// Grid: (page slots of each sequence) x (head groups) x (K, V).  Threads:
+// Grid: (K, V) x (page slots of each sequence) x (head groups).  Threads:
 // page_size * D / 32.
-template <class T, int D, bool ODD>
+template <class T, int D, int MODE>
 __global__ __launch_bounds__(4 * D) void append_pages_kernel(Cache c, AppendArgs a, int page_slots, int groups) {
+    constexpr bool ODD = MODE == kOdd;
     constexpr int U = ODD ? 3 : 2;  // groups of 16 values per thread
     __shared__ unsigned red[2][16];
     const int tid = threadIdx.x, nt = blockDim.x, waves = (nt + 63) >> 6;
     int id = blockIdx.x;
     const int hg = id % groups;
     id /= groups;
-    const bool is_v = id & 1;
-    id >>= 1;
+    const bool is_v = id >= c.B * page_slots;  // last: K's workgroups, with queries, have more to do
+    if (is_v) id -= c.B * page_slots;
     const int b = id / page_slots, slot = id % page_slots;
     const Seq s = sequence(c, b);
     if (s.n == 0) return;
@@ -284,20 +298,19 @@ __global__ __launch_bounds__(4 * D) void append_pages_kernel(Cache c, AppendArgs
             const int tok = lo + (k >> 2) * 16 + (k & 3);
             fresh |= (tok >= t0 && tok < t1) << k;
         }
-        float x[8][4], nx[8][4];
-        auto load = [&](int h, float (*to)[4]) {
+        float x[8][4];
+        auto load = [&](int h) {
             const T* v = static_cast<const T*>(a.v) + h * a.v_hs + d0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 if (fresh >> k & 1)
-                    load4(v + (row0 + lo + (k >> 2) * 16 + (k & 3)) * a.v_ts, to[k]);
+                    load4(v + (row0 + lo + (k >> 2) * 16 + (k & 3)) * a.v_ts, x[k]);
                 else
-                    to[k][0] = to[k][1] = to[k][2] = to[k][3] = 0.f;
+                    x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
             }
         };
-        if (h0 < h1) load(h0, x);
         for (int h = h0; h < h1; ++h) {
-            if (h + 1 < h1) load(h + 1, nx);
+            load(h);
             uint8_t* codes = c.v + page * c.page_stride + h * c.head_stride;
             float* sp = c.vs + page * c.s_page_stride + h * c.s_head_stride;
             const float old = t0 > 0 ? *sp : 0.f;
@@ -332,17 +345,13 @@ __global__ __launch_bounds__(4 * D) void append_pages_kernel(Cache c, AppendArgs
                 }
             }
             if (tid == 0) *sp = sc.scale;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[k][j] = nx[k][j];
         }
         return;
     }
 
     const int half = a.rot >> 1;
     const int per_row = ODD ? ((half + 7) >> 3) + ((D - a.rot + 15) >> 4) : D / 16;
-    Group<ODD> gr[U];
+    Group<MODE> gr[U];
     int tok[U];
     bool live[U];
     float cs[U][8], sn[U][8];
@@ -403,7 +412,8 @@ __global__ __launch_bounds__(256) void append_token_kernel(Cache c, AppendArgs a
     const int per = 2 * c.H + (a.q ? a.Hq : 0);
     const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (item >= (int64_t)c.B * per) return;
-    const int b = __builtin_amdgcn_readfirstlane((int)(item / per)), x = __builtin_amdgcn_readfirstlane((int)(item % per));
+    const int b = __builtin_amdgcn_readfirstlane((int)(item / per));
+    const int x = __builtin_amdgcn_readfirstlane((int)(item % per));
     const int lane = threadIdx.x & 63;
     const bool on = D >= 64 || lane < D;
     const bool is_q = x >= 2 * c.H, is_v = !is_q && x >= c.H;
@@ -552,10 +562,10 @@ hipError_t append_d(const Cache& c, const AppendArgs& a, hipStream_t s) {
     const int64_t grid = (int64_t)c.B * slots * 2 * groups;
     if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidConfiguration;
     const dim3 nt(ps * D / 32 < 64 ? 64 : ps * D / 32);  // a whole wave: idle lanes have no token
-    if (a.rot && !a.interleaved && a.rot % 16)
-        hipLaunchKernelGGL((append_pages_kernel<T, D, true>), dim3((unsigned)grid), nt, 0, s, c, a, slots, groups);
-    else
-        hipLaunchKernelGGL((append_pages_kernel<T, D, false>), dim3((unsigned)grid), nt, 0, s, c, a, slots, groups);
+    auto kern = !a.rot || a.interleaved ? append_pages_kernel<T, D, kPairs>
+                : a.rot % 16            ? append_pages_kernel<T, D, kOdd>
+                                        : append_pages_kernel<T, D, kHalves>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), nt, 0, s, c, a, slots, groups);
     return hipGetLastError();
 }
 
