@@ -365,30 +365,30 @@ __global__ __launch_bounds__(TW * 64, D <= 128 ? 2 : 1) void attn_tiles_kernel(C
 // w, 2w where it goes on), and a second kernel joins them.  Lengths are on the
 // device, so every workgroup sums them up by itself.
 constexpr int kMinShare = 4;  // stages
-constexpr int kPlan = TW * 64;
+constexpr int kPlan = TW * 64;    // threads
 
 struct Plan {
-    int pre[kPlan];   // stages of one head before thread t's items
-    int wave_sum[TW];
-    int found[3];     // item, its first stage, its stages
+    int64_t wave_sum[TW];
+    int64_t at;      // first stage of the item found
+    int item, n;     // the item, its stages
 };
 
 struct Shares {
-    int per_head, chunk;
-    int64_t total, share;
-    int my_pre, my_sum;
+    int chunk;
+    int64_t per_head, total, share;  // stages: more than 2^31 in a prompt of 4 M tokens
+    int64_t my_pre, my_sum;
     // Items are (sequence, row block); thread t sums items [t * chunk, ...).
     __device__ __forceinline__ void init(const Cache& c, int G, int row_blocks, int count, Plan& pl) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         const int items = c.B * row_blocks;
-        chunk = (items + kPlan - 1) / kPlan;
+        chunk = items / kPlan + 1;
         my_sum = 0;
-        for (int i = tid * chunk; i < min(items, (tid + 1) * chunk); ++i)
-            my_sum += block_stages(c, G, i / row_blocks, i % row_blocks);
-        int inc = my_sum;
+        for (int64_t i = (int64_t)tid * chunk, e = min((int64_t)items, i + chunk); i < e; ++i)
+            my_sum += block_stages(c, G, (int)(i / row_blocks), (int)(i % row_blocks));
+        int64_t inc = my_sum;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(inc, d);
+            const int64_t x = __shfl_up((long long)inc, d);
             if (lane >= d) inc += x;
         }
         if (lane == 63) pl.wave_sum[wave] = inc;
@@ -400,22 +400,23 @@ struct Shares {
             if (w < wave) my_pre += pl.wave_sum[w];
             per_head += pl.wave_sum[w];
         }
-        total = (int64_t)per_head * c.H;
+        total = per_head * c.H;
         share = max((total + count - 1) / count, (int64_t)kMinShare);
     }
     // The item that holds stage p of its head: pl.found, for all threads.
-    __device__ __forceinline__ void find(const Cache& c, int G, int row_blocks, int p, Plan& pl) const {
+    __device__ __forceinline__ void find(const Cache& c, int G, int row_blocks, int64_t p, Plan& pl) const {
         __syncthreads();
         if (p >= my_pre && p < my_pre + my_sum) {
-            int at = my_pre, i = threadIdx.x * chunk, n = block_stages(c, G, i / row_blocks, i % row_blocks);
+            int64_t at = my_pre;
+            int i = threadIdx.x * chunk, n = block_stages(c, G, i / row_blocks, i % row_blocks);
             while (p >= at + n) {
                 at += n;
                 ++i;
                 n = block_stages(c, G, i / row_blocks, i % row_blocks);
             }
-            pl.found[0] = i;
-            pl.found[1] = at;
-            pl.found[2] = n;
+            pl.item = i;
+            pl.at = at;
+            pl.n = n;
         }
         __syncthreads();
     }
@@ -433,16 +434,15 @@ __global__ __launch_bounds__(TW * 64, D <= 128 ? 2 : 1) void attn_shares_kernel(
     const int64_t end = min(sh.total, p + sh.share);
     int4 join = {0, 0, 0, -1};  // (sequence, head, row block, last share) of a block that begins here and goes on
     while (p < end) {
-        const int h = (int)(p / sh.per_head), in_head = (int)(p % sh.per_head);
+        const int h = (int)(p / sh.per_head);
+        const int64_t in_head = p % sh.per_head;
         sh.find(c, G, row_blocks, in_head, pl);
-        const int item = __builtin_amdgcn_readfirstlane(pl.found[0]);
-        const int at = __builtin_amdgcn_readfirstlane(pl.found[1]);
-        const int n = __builtin_amdgcn_readfirstlane(pl.found[2]);
+        const int item = __builtin_amdgcn_readfirstlane(pl.item), n = __builtin_amdgcn_readfirstlane(pl.n);
         Piece pc;
         pc.b = item / row_blocks;
         pc.h = h;
         pc.rb = item % row_blocks;
-        pc.s0 = in_head - at;
+        pc.s0 = __builtin_amdgcn_readfirstlane((int)(in_head - pl.at));
         pc.s1 = (int)min((int64_t)n, pc.s0 + (end - p));
         pc.slot = pc.s0 > 0 ? 2 * w : pc.s1 < n ? 2 * w + 1 : -1;
         if (pc.slot & 1 && pc.slot > 0) join = {pc.b, h, pc.rb, (int)((p + n - 1) / sh.share)};
