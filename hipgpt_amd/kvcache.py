@@ -241,13 +241,15 @@ def _attention(name, rows, cache, batch, q, out, out_dtype, scale, num_splits, w
     odt = _dtype("out", out)
     if num_splits is None:
         num_splits = default_splits(batch.size, T, batch.max_new, Hq, H, D, out.dtype,
-                                    batch.max_len or batch.capacity(cache))
+                                    min(batch.max_len or batch.capacity(cache), 0x7fffffff))
     ns = int(num_splits)
     wp = nbytes = 0
     if ns > 1:
         if workspace is None:
             need = workspace_bytes(batch.size, T, batch.max_new, Hq, H, D, out.dtype, ns)
             workspace = mine[1] = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous, on {dev}")
         wp, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     rc = getattr(_lib.lib(), name)(
         cache._ref, batch._ref, *rows, q.data_ptr(), out.data_ptr(), Hq, *qs, *os_,

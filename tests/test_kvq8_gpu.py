@@ -55,7 +55,7 @@ class Case:
             for j in range(-(-n // ps)):
                 for w in "kv":
                     self.scale[w][self.table[b, j]] = rng.uniform(0.01, 0.03, H)
-        ku, vu = R.codes_to_pool(np.stack([self.codes["k"], self.codes["v"]])[0])[0], R.codes_to_pool(self.codes["v"])[1]
+        ku, vu = R.codes_to_pool(self.codes["k"])[0], R.codes_to_pool(self.codes["v"])[1]
         # pages `pad` bytes apart, scales in a wider array
         buf = torch.from_numpy(rng.integers(0, 256, (2, pages, H * ps * D + pad), dtype=np.uint8)).cuda()
         pools = buf[:, :, :H * ps * D].view(2, pages, H, ps, D)
@@ -657,7 +657,8 @@ def test_captured_prefill_replays(dev, splits):
     b = c.batch(lens, new)
     q, k, v = (normal(c.rng, "bf16", sum(new), h, D)[0] for h in (4, H, H))
     qr, out = torch.empty_like(q), torch.empty(sum(new), 4, D, device="cuda")
-    ws = torch.empty(max(1, K.workspace_bytes(2, sum(new), n, 4, H, D, torch.float32, splits)), dtype=torch.uint8, device="cuda")
+    need = K.workspace_bytes(2, sum(new), n, 4, H, D, torch.float32, splits)
+    ws = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
     f = K.rope_freqs(D)
 
     def step():
@@ -753,3 +754,30 @@ def test_pools_by_head(dev):
     check_append(c, lens, new, {"k": k64, "v": v64}, 0, False, before, c.state())
     got = host(K.prefill(c.cache, c.batch(lens, new), q))
     check_attention(c, got, q64, lens, new, 2, 0.125, "f32", c.state())
+
+
+def test_workspace_refusals(dev):
+    c = Case(161, [2000], [2000], 2, 64, 64)
+    q, _ = normal(c.rng, "f32", 1, 2, 64)
+    need = K.workspace_bytes(1, 1, 1, 2, 2, 64, torch.float32, 4)
+    ws = torch.empty(2 * need, dtype=torch.uint8, device="cuda")
+    b = c.batch([2000])
+    for bad in (torch.empty(need, dtype=torch.uint8), ws[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            K.decode(c.cache, b, q, num_splits=4, workspace=bad)
+    with pytest.raises(Exception, match="(?i)workspace"):
+        K.decode(c.cache, b, q, num_splits=4, workspace=ws[:need - 1])
+
+
+def test_table_past_int_tokens(dev):
+    """A table whose row holds 2^31 tokens and more, and a max_len beyond int: the default split."""
+    c = Case(162, [2900], [2900], 2, 128, 64)
+    q, q64 = normal(c.rng, "f32", 1, 2, 64)
+    table = torch.zeros(1, (1 << 24) + 1, dtype=torch.int32, device="cuda")
+    table[0, :c.table.shape[1]] = torch.from_numpy(c.table[0]).cuda()
+    lens = torch.tensor([2900], dtype=torch.int32, device="cuda")
+    k, v = c.rows("k", 0, 2900), c.rows("v", 0, 2900)
+    want = R.attend(q64, k, v, 1, 0.125, 2899)
+    for max_len in (None, 1 << 31, 1 << 33):
+        got = host(K.decode(c.cache, K.Batch(table, lens, max_len=max_len), q))
+        assert np.abs(got - want).max() <= R.f32_tol(v)
