@@ -99,7 +99,8 @@ __device__ __forceinline__ int q_dim(int s, int q) {
 // its keys; the four waves take every fourth 32-token tile and are joined in
 // LDS.  TERMS: columns per row (2: q and p as two fp16 terms).
 template <int D, int TERMS, class TI, class TO>
-__global__ __launch_bounds__(NW * 64, D <= 64 ? 4 : D == 128 ? 3 : 2) void attn_rows_kernel(Cache c, AttnArgsQ8 a, int row_blocks) {
+__global__ __launch_bounds__(NW * 64, D <= 64 ? 4 : D == 128 ? 3 : 2) void attn_rows_kernel(Cache c, AttnArgsQ8 a,
+                                                                                           int row_blocks) {
     constexpr int RPB = 16 / TERMS;  // rows per block
     __shared__ float s_m[NW][16], s_l[NW][16], s_ref[NW];
     __shared__ __attribute__((aligned(16))) float s_o[NW][16][D + 4];
@@ -392,7 +393,7 @@ hipError_t launch_rows(const Cache& c, const AttnArgsQ8& a, hipStream_t s) {
 
 template <int D>
 hipError_t launch_dim(const Cache& c, const AttnArgsQ8& a, int dtype, int out_dtype, hipStream_t s) {
-        hipError_t e;
+    hipError_t e;
     if (tiles_for(c.B, c.max_new, a.Hq, c.H, out_dtype)) return launch_tiles(c, a, dtype, out_dtype, s);
     if (dtype == kF32)
         e = launch_rows<D, 2, float, float>(c, a, s);
